@@ -819,3 +819,268 @@ def wmma_splitk_partials(Q, K, V, batch_size, N_latent, N_input, D, num_splits, 
                                          N_input, D, 1, 0, num_splits, 142, bf16,
                                          keep_partials=True)
     return out, parts
+
+
+# ---------------------------------------------------------------------------
+# Attention over a key/value cache (additive)
+# ---------------------------------------------------------------------------
+
+class RopeArgs(ctypes.Structure):
+    """xattn_rope: device frequencies, amplitude, rot_dim, interleaved."""
+    _fields_ = [("freqs", _P), ("amplitude", ctypes.c_float), ("rot_dim", _I),
+                ("interleaved", _I)]
+
+
+class CacheArgs(ctypes.Structure):
+    """xattn_kv_cache: device pages of keys and of values and their shape."""
+    _fields_ = [("k", _P), ("v", _P), ("dtype", _I), ("num_pages", _I), ("kv_heads", _I),
+                ("page_size", _I), ("dim", _I)]
+
+
+class BatchArgs(ctypes.Structure):
+    """xattn_batch: device descriptors of a ragged batch and its sizes."""
+    _fields_ = [("q_starts", _P), ("kv_lens", _P), ("page_table", _P), ("batch", _I),
+                ("table_width", _I), ("tokens", _I), ("max_q_len", _I), ("max_kv_len", _I)]
+
+
+class PrefixArgs(ctypes.Structure):
+    """xattn_prefix: device page numbers, how many, and the keys on them."""
+    _fields_ = [("pages", _P), ("num_listed", _I), ("len", _I)]
+
+
+_LL = ctypes.c_longlong
+_CACHE, _BATCH = ctypes.POINTER(CacheArgs), ctypes.POINTER(BatchArgs)
+_ROPE, _PREFIX = ctypes.POINTER(RopeArgs), ctypes.POINTER(PrefixArgs)
+# q, q stride, out, out stride, heads, scale, causal, scratch, bytes, stream
+_ATTEND_TAIL = [_P, _LL, _P, _LL, _I, ctypes.c_float, _I, _P, ctypes.c_size_t, _P]
+
+HAS_CACHE = (
+    _bind_optional("launch_rope_kernel",
+                   [_P, _P, _P, _ROPE, _I, _I, _I, _I, _LL, _LL, _I, _P])
+    and _bind_optional("launch_cache_append_kernel",
+                       [_CACHE, _BATCH, _P, _LL, _P, _LL, _P, _LL, _P, _LL, _I, _P, _ROPE, _P])
+    and _bind_optional("launch_cache_attention_kernel", [_CACHE, _BATCH] + _ATTEND_TAIL)
+    and _bind_optional("launch_prefix_attention_kernel",
+                       [_CACHE, _BATCH, _PREFIX] + _ATTEND_TAIL))
+if HAS_CACHE:
+    lib.xattn_rope_frequencies.argtypes = [ctypes.POINTER(ctypes.c_double), _I, ctypes.c_double,
+                                           _I, ctypes.c_double, _I, ctypes.c_double,
+                                           ctypes.c_double]
+    lib.xattn_rope_frequencies.restype = ctypes.c_int
+    lib.xattn_cache_attention_scratch.argtypes = [_CACHE, _BATCH, _PREFIX, _I]
+    lib.xattn_cache_attention_scratch.restype = ctypes.c_size_t
+
+PRECISIONS = {"fp32": 0, "fp16": 1, "bf16": 2}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+
+
+def _require_cache():
+    if not HAS_CACHE:
+        raise RuntimeError("this kernels.so does not export the cache operators")
+
+
+def _precision(precision):
+    if precision not in PRECISIONS:
+        raise ValueError(f"precision {precision!r} is not fp32, fp16 or bf16")
+    return PRECISIONS[precision]
+
+
+def _encode(x, precision):
+    """float32 values -> contiguous array of the type's bit patterns."""
+    if precision == "bf16":
+        return _to_bf16_bits(x)
+    return np.ascontiguousarray(x, dtype=np.float16 if precision == "fp16" else np.float32)
+
+
+def _decode(x, precision):
+    """What _encode made -> float32 values."""
+    if precision == "bf16":
+        return (x.astype(np.uint32) << 16).view(np.float32)
+    return x.astype(np.float32)
+
+
+def _bits_type(precision):
+    return {"fp32": np.float32, "fp16": np.float16, "bf16": np.uint16}[precision]
+
+
+def rope_frequencies(rot_dim, base=10000.0, scaling="none", factor=1.0, trained_len=0,
+                     slow_turns=1.0, fast_turns=32.0):
+    """Turns per position of the rot_dim / 2 rotated pairs (float64), for a
+    context stretched by ``factor``: "linear" divides every frequency by it,
+    "base" raises the base so that the slowest pair is, and "parts" divides those
+    that make up to slow_turns turns over trained_len positions, keeps those
+    that make fast_turns or more, and blends in between (where 0.1 ln(factor) +
+    1 is the usual ``amplitude`` of the rotation)."""
+    _require_cache()
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"scaling {scaling!r} is not one of {', '.join(ROPE_SCALINGS)}")
+    freqs = np.zeros(max(int(rot_dim) // 2, 1), np.float64)
+    lib.xattn_rope_frequencies(freqs.ctypes.data_as(ctypes.POINTER(ctypes.c_double)),
+                               int(rot_dim), base, ROPE_SCALINGS[scaling], factor,
+                               int(trained_len), slow_turns, fast_turns)
+    _lib_error_check("xattn_rope_frequencies")
+    return freqs[:int(rot_dim) // 2]
+
+
+class Rope:
+    """A rotation for run_rope and PagedCache.append: ``freqs`` (turns per
+    position of each pair, see rope_frequencies), ``amplitude``, and whether
+    pairs are interleaved (2i, 2i + 1) or halves (i, i + rot_dim / 2).  Keeps the
+    frequencies on the device until ``close()`` or the end of a with block."""
+
+    def __init__(self, freqs, amplitude=1.0, interleaved=False):
+        _require_cache()
+        freqs = np.ascontiguousarray(freqs, np.float64)
+        self._freqs = DeviceBuffer.holding(freqs)
+        self.args = RopeArgs(self._freqs.ptr.value, amplitude, 2 * freqs.size, int(interleaved))
+
+    def close(self):
+        self._freqs.close()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+
+def run_rope(x, positions, rope, inverse=False, precision="fp32"):
+    """One launch_rope_kernel call on host arrays: x [tokens, heads, dim] with
+    ``rope`` applied at ``positions`` [tokens], or with ``inverse`` the
+    gradient of x from that of the rotated values.  x is rounded to
+    ``precision``, the result returned as float32."""
+    _require_cache()
+    code = _precision(precision)
+    host = _encode(np.asarray(x, np.float32), precision)
+    tokens, heads, dim = host.shape
+    positions = np.ascontiguousarray(positions, np.int32)
+    if positions.shape != (tokens,):
+        raise ValueError(f"positions of shape {positions.shape} for {tokens} tokens")
+    with DeviceBuffer.holding(host) as dx, DeviceBuffer(host.nbytes) as dy, \
+            DeviceBuffer.holding(positions) as dp:
+        lib.launch_rope_kernel(dx.ptr, dy.ptr, dp.ptr, ctypes.byref(rope.args), code, tokens,
+                               heads, dim, heads * dim, heads * dim, int(inverse), _NULL_STREAM)
+        _raise_launch_errors("launch_rope_kernel")
+        _hip_check(cudart.hipDeviceSynchronize(), "launch_rope_kernel: waiting for the kernel")
+        return _decode(dy.download(host.shape, host.dtype), precision)
+
+
+class PagedCache:
+    """A cache of keys and values on pages of the device, and the launches
+    that fill and read it, on host arrays (every call copies its operands, as
+    the run_* functions do; programs with data on the device call the
+    launchers of ``lib`` with ``args``).
+
+    A batch is ragged: sequence b owns the token rows q_starts[b] to
+    q_starts[b + 1] of k, v and q, and kv_lens[b] keys, its new tokens' last,
+    on the pages page_table[b] lists.  The caller hands out the pages."""
+
+    def __init__(self, num_pages, page_size, kv_heads, dim, precision="fp32"):
+        _require_cache()
+        self.precision, self.code = precision, _precision(precision)
+        self.shape = (int(num_pages), int(kv_heads), int(page_size), int(dim))
+        if min(self.shape) < 1:
+            raise ValueError(f"a cache of shape {self.shape}")
+        nbytes = int(np.prod(self.shape, dtype=np.int64)) * np.dtype(_bits_type(precision)).itemsize
+        self._owned = contextlib.ExitStack()
+        try:
+            self._k = self._owned.enter_context(DeviceBuffer(nbytes)).zero()
+            self._v = self._owned.enter_context(DeviceBuffer(nbytes)).zero()
+        except Exception:
+            self._owned.close()
+            raise
+        self.args = CacheArgs(self._k.ptr.value, self._v.ptr.value, self.code, num_pages,
+                              kv_heads, page_size, dim)
+
+    def close(self):
+        self._owned.close()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def pages(self):
+        """Host copies (keys, values) [num_pages, kv_heads, page_size, dim], float32."""
+        kind = _bits_type(self.precision)
+        return tuple(_decode(b.download(self.shape, kind), self.precision)
+                     for b in (self._k, self._v))
+
+    def _batch(self, owned, tokens, q_starts, kv_lens, page_table):
+        q_starts, kv_lens = (np.ascontiguousarray(a, np.int32) for a in (q_starts, kv_lens))
+        page_table = np.ascontiguousarray(page_table, np.int32)
+        batch = kv_lens.size
+        if q_starts.shape != (batch + 1,) or page_table.ndim != 2 or len(page_table) != batch:
+            raise ValueError(f"q_starts {q_starts.shape}, kv_lens {kv_lens.shape} and page_table "
+                             f"{page_table.shape} do not describe one batch")
+        on = [owned.enter_context(DeviceBuffer.holding(a)) for a in (q_starts, kv_lens, page_table)]
+        longest = int(max(np.diff(q_starts), default=0))
+        return BatchArgs(*(b.ptr.value for b in on), batch, page_table.shape[1], tokens,
+                         max(longest, 0), max(int(max(kv_lens, default=0)), 0))
+
+    def _tokens(self, x, heads, what):
+        x = np.asarray(x, np.float32)
+        if x.ndim != 3 or x.shape[2] != self.shape[3] or (heads and x.shape[1] != heads):
+            raise ValueError(f"{what} of shape {x.shape} for a cache of shape {self.shape}")
+        return _encode(x, self.precision)
+
+    def append(self, k, v, q_starts, kv_lens, page_table, q=None, rope=None, positions=None):
+        """launch_cache_append_kernel: k and v [tokens, kv_heads, dim] into the
+        cache, k rotated by ``rope`` at ``positions`` (default: the cache
+        positions).  With q [tokens, heads, dim], returns it rotated alike."""
+        k, v = (self._tokens(a, self.shape[1], n) for a, n in ((k, "k"), (v, "v")))
+        q = None if q is None else self._tokens(q, None, "q")
+        if len(v) != len(k) or (q is not None and len(q) != len(k)):
+            raise ValueError("k, v and q have to hold the same tokens")
+        if positions is not None:
+            positions = np.ascontiguousarray(positions, np.int32)
+            if positions.shape != (len(k),):
+                raise ValueError(f"positions of shape {positions.shape} for {len(k)} tokens")
+        row = self.shape[1] * self.shape[3]
+        with contextlib.ExitStack() as owned:
+            batch = self._batch(owned, len(k), q_starts, kv_lens, page_table)
+            dk, dv = (owned.enter_context(DeviceBuffer.holding(a)) for a in (k, v))
+            dq = None if q is None else owned.enter_context(DeviceBuffer.holding(q))
+            dp = None if positions is None else owned.enter_context(DeviceBuffer.holding(positions))
+            heads = 0 if q is None else q.shape[1]
+            q_row = heads * self.shape[3]
+            lib.launch_cache_append_kernel(
+                ctypes.byref(self.args), ctypes.byref(batch), dk.ptr, row, dv.ptr, row,
+                dq and dq.ptr, q_row, dq and dq.ptr, q_row, heads, dp and dp.ptr,
+                None if rope is None else ctypes.byref(rope.args), _NULL_STREAM)
+            _raise_launch_errors("launch_cache_append_kernel")
+            _hip_check(cudart.hipDeviceSynchronize(),
+                       "launch_cache_append_kernel: waiting for the kernel")
+            return None if q is None else _decode(dq.download(q.shape, q.dtype), self.precision)
+
+    def attend(self, q, q_starts, kv_lens, page_table, scale=None, causal=True,
+               prefix_pages=None, prefix_len=0):
+        """launch_cache_attention_kernel, or with prefix_pages
+        launch_prefix_attention_kernel: q [tokens, heads, dim] -> output of the
+        same shape, float32.  scale defaults to 1/sqrt(dim)."""
+        if self.shape[3] not in (64, 128, 256, D_MODEL):
+            raise DesignLimited(f"cache attention is built for heads of 64, 128, 256 or {D_MODEL} "
+                                f"(got {self.shape[3]})")
+        q = self._tokens(q, None, "q")
+        tokens, heads, dim = q.shape
+        scale = dim ** -0.5 if scale is None else scale
+        with contextlib.ExitStack() as owned:
+            batch = self._batch(owned, tokens, q_starts, kv_lens, page_table)
+            launch, before, prefix = lib.launch_cache_attention_kernel, (), None
+            if prefix_pages is not None:
+                prefix_pages = np.ascontiguousarray(prefix_pages, np.int32)
+                on = owned.enter_context(DeviceBuffer.holding(prefix_pages))
+                prefix = ctypes.byref(PrefixArgs(on.ptr.value, prefix_pages.size, prefix_len))
+                launch, before = lib.launch_prefix_attention_kernel, (prefix,)
+            cache, batch = ctypes.byref(self.args), ctypes.byref(batch)
+            need = lib.xattn_cache_attention_scratch(cache, batch, prefix, heads)
+            dq = owned.enter_context(DeviceBuffer.holding(q))
+            out = owned.enter_context(DeviceBuffer(q.nbytes)).zero()
+            scratch = owned.enter_context(DeviceBuffer(need))
+            launch(cache, batch, *before, dq.ptr, heads * dim, out.ptr, heads * dim, heads,
+                   scale, int(causal), scratch.ptr, need, _NULL_STREAM)
+            _raise_launch_errors(launch.__name__)
+            _hip_check(cudart.hipDeviceSynchronize(),
+                       f"{launch.__name__}: waiting for the kernel")
+            return _decode(out.download(q.shape, q.dtype), self.precision)

@@ -42,6 +42,7 @@
 #ifndef XATTN_H
 #define XATTN_H
 
+#include <stddef.h>
 #include <stdint.h>
 #include <hip/hip_runtime_api.h>
 
@@ -200,6 +201,159 @@ void launch_wmma_plan_kernel(int bf16, const uint16_t* Q, const uint16_t* K,
                              int N_latent, int N_input, int dim,
                              int latents_per_workgroup, int column_parts,
                              int num_splits, hipStream_t stream);
+
+/* ---- attention over a key/value cache (additive) ----------------------- */
+/*
+ * No reference counterpart: the operators of a model that is served with its
+ * keys and values in a paged cache.  Heads are grouped: heads query heads
+ * share kv_heads key/value heads (heads a multiple of kv_heads; query head h
+ * reads kv head h / (heads / kv_heads)).
+ *
+ * All of them only enqueue work on `stream`, never allocate, never
+ * synchronise, may be captured into a graph, and work on the current device.
+ * Arguments that the host can judge are refused before anything is launched,
+ * as for the entry points above.  The contents of device arrays are checked
+ * by the kernels, which never read or write out of bounds for a wrong
+ * length, position or page number: what becomes of such a sequence stands at
+ * each call.  The structures below are read during the call only.
+ */
+
+/* Element type of a cache and of the tensors that go with it. */
+enum { XATTN_F32 = 0, XATTN_F16 = 1, XATTN_BF16 = 2 };
+
+/* A rotation of pairs of a head's first rot_dim elements by the token's
+ * position: pair i by the angle 2 pi * position * freqs[i], its cosine and
+ * sine times amplitude.  Pairs are (i, i + rot_dim / 2), or with interleaved
+ * != 0 (2 i, 2 i + 1); elements from rot_dim on are left as they are.  Angles
+ * are reduced in 64 bits, so far positions lose nothing. */
+typedef struct xattn_rope {
+    const double* freqs; /* device, [rot_dim / 2]: turns per position */
+    float amplitude;     /* 1 unless the scaling asks for another */
+    int rot_dim;         /* even, 0 .. dim */
+    int interleaved;
+} xattn_rope;
+
+/* Pages of keys and values, [num_pages][kv_heads][page_size][dim] each, of
+ * type dtype, 16-byte aligned.  page_size is any number >= 1. */
+typedef struct xattn_kv_cache {
+    void* k;
+    void* v;
+    int dtype;
+    int num_pages;
+    int kv_heads;
+    int page_size;
+    int dim;
+} xattn_kv_cache;
+
+/* A ragged batch.  Sequence b owns the token rows q_starts[b] ..
+ * q_starts[b + 1] - 1 of the token tensors and has kv_lens[b] keys, those of
+ * its own new tokens last: its token i stands at cache position
+ * kv_lens[b] - (q_starts[b + 1] - q_starts[b]) + i.  Position p lies in slot
+ * p % page_size of page page_table[b][p / page_size].  Token rows before
+ * q_starts[0] and from q_starts[batch] on belong to nobody and are left as
+ * they are. */
+typedef struct xattn_batch {
+    const int* q_starts;   /* device, [batch + 1], not decreasing */
+    const int* kv_lens;    /* device, [batch] */
+    const int* page_table; /* device, [batch][table_width] */
+    int batch;
+    int table_width;
+    int tokens;     /* rows of the token tensors, >= q_starts[batch] */
+    int max_q_len;  /* at least the longest sequence's new tokens */
+    int max_kv_len; /* about the longest kv_lens: the work is divided by it */
+} xattn_batch;
+
+/* Keys that every sequence of a batch sees before its own: positions 0 ..
+ * len - 1 on pages[0 .. num_listed - 1], len <= num_listed * page_size. */
+typedef struct xattn_prefix {
+    const int* pages; /* device, [num_listed] */
+    int num_listed;
+    int len;
+} xattn_prefix;
+
+enum {
+    XATTN_ROPE_PLAIN = 0,  /* base^(-2 i / rot_dim) / (2 pi) turns a position  */
+    XATTN_ROPE_LINEAR = 1, /* the same / factor                                */
+    XATTN_ROPE_BASE = 2,   /* base * factor^(rot_dim / (rot_dim - 2)) as base  */
+    XATTN_ROPE_PARTS = 3   /* a blend of PLAIN and LINEAR, by the turns that a */
+                           /* pair makes over trained_len positions: LINEAR    */
+                           /* up to slow_turns, PLAIN from fast_turns on,      */
+                           /* linear in between                                */
+};
+/* Fills the host array freqs[rot_dim / 2] with turns per position.  factor
+ * is the stretch of the context; trained_len, slow_turns and fast_turns
+ * count for XATTN_ROPE_PARTS only.  Returns XATTN_OK, or the error it also
+ * records: rot_dim odd or negative, base or factor not positive and finite, an
+ * unknown scaling, XATTN_ROPE_BASE with rot_dim 2, and for XATTN_ROPE_PARTS
+ * trained_len < 1 or not 0 <= slow_turns < fast_turns. */
+int xattn_rope_frequencies(double* freqs, int rot_dim, double base, int scaling, double factor,
+                           int trained_len, double slow_turns, double fast_turns);
+
+/* y = x with its rotary positions applied (inverse == 0), or with the
+ * transposed rotation (inverse != 0): the gradient of x from that of y.
+ * x and y [tokens][heads][dim] of type dtype, token rows x_stride and
+ * y_stride elements apart (>= heads * dim); positions device int [tokens],
+ * any values.  y may be x (with the same stride), but may not overlap it
+ * otherwise.  dim is any number >= 1. */
+void launch_rope_kernel(const void* x, void* y, const int* positions, const xattn_rope* rope,
+                        int dtype, int tokens, int heads, int dim, long long x_stride,
+                        long long y_stride, int inverse, hipStream_t stream);
+
+/* Puts the new tokens' keys and values, k and v [tokens][kv_heads][dim] with
+ * rows k_stride and v_stride elements apart, into the cache, the keys rotated
+ * by rope (NULL: as they are) at positions[token] (NULL: the token's cache
+ * position).  With q not NULL also writes q_out [tokens][heads][dim], the
+ * same tokens' queries rotated alike (q_out may be q with the same stride).
+ * dim is any number >= 1; heads counts for q only.
+ * A token whose cache position is negative, beyond its row of page_table or
+ * on a page number outside 0 .. num_pages - 1 is not put into the cache.  Two
+ * tokens of one call that share a slot leave either in it. */
+void launch_cache_append_kernel(const xattn_kv_cache* cache, const xattn_batch* batch,
+                                const void* k, long long k_stride, const void* v,
+                                long long v_stride, const void* q, long long q_stride,
+                                void* q_out, long long q_out_stride, int heads,
+                                const int* positions, const xattn_rope* rope,
+                                hipStream_t stream);
+
+/* Bytes of device scratch that the two launchers below need for this cache,
+ * batch (its sizes alone count), prefix (NULL: none) and number of query
+ * heads on the current device; 0 where they need none, or where they would
+ * refuse the sizes. */
+size_t xattn_cache_attention_scratch(const xattn_kv_cache* cache, const xattn_batch* batch,
+                                     const xattn_prefix* prefix, int heads);
+
+/* out = softmax(scale * q k^T) v over the cache: every token of sequence b
+ * sees the keys up to its own cache position (causal != 0), or all kv_lens[b]
+ * (causal == 0).  q and out [tokens][heads][dim] of the cache's type, rows
+ * q_stride and out_stride elements apart (>= heads * dim); all pointers
+ * 16-byte aligned, strides multiples of 16 bytes.  Keys that a token does not
+ * see do not count, whatever they hold (infinities and NaN included); a token
+ * that sees none gets zeros.  dim 64, 128, 256 or 768.  out may not overlap q.
+ * The tokens of a sequence come out as NaN if its length is negative or
+ * beyond its row of page_table, or if a page that they see has a number
+ * outside 0 .. num_pages - 1; those past max_q_len are left as they are.
+ * scratch: scratch_bytes >= xattn_cache_attention_scratch bytes, 16-byte
+ * aligned, of this call alone until it has finished: calls (and replays of
+ * graphs) that may overlap need scratch of their own.  Its contents need no
+ * initialisation.  Sums and softmax statistics are kept in 32 bits, weights
+ * rounded to the cache's type for the product with v; results do not depend
+ * on the order in which workgroups run. */
+void launch_cache_attention_kernel(const xattn_kv_cache* cache, const xattn_batch* batch,
+                                   const void* q, long long q_stride, void* out,
+                                   long long out_stride, int heads, float scale, int causal,
+                                   void* scratch, size_t scratch_bytes, hipStream_t stream);
+
+/* The same for a batch whose sequences share a prefix: every token sees all
+ * prefix->len keys of the prefix, and its sequence's own as above (kv_lens and
+ * page_table count those only; kv_lens[b] may be 0 with new tokens that are
+ * not in the cache).  The prefix's keys and values are read once for all
+ * sequences, not once for each.  A page number outside 0 .. num_pages - 1
+ * among the prefix's pages makes the whole output NaN. */
+void launch_prefix_attention_kernel(const xattn_kv_cache* cache, const xattn_batch* batch,
+                                    const xattn_prefix* prefix, const void* q,
+                                    long long q_stride, void* out, long long out_stride,
+                                    int heads, float scale, int causal, void* scratch,
+                                    size_t scratch_bytes, hipStream_t stream);
 
 /* ---- library status / device queries (additive) ----------------------- */
 
