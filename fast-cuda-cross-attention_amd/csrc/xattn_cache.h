@@ -78,6 +78,12 @@ struct Attention {
 size_t attention_scratch(const Attention& a);
 bool launch_attention(const Attention& a, void* scratch, hipStream_t stream);
 
+// Four elements of a row.
+template <typename T>
+struct alignas(4 * sizeof(T)) Piece4 {
+    T e[4];
+};
+
 // Elements of a cache's type in 32 bits and back (rounded to nearest even).
 template <typename T> __device__ inline float to_f32(T x) { return (float)x; }
 template <typename T> __device__ inline T from_f32(float x) { return (T)x; }

@@ -1,86 +1,697 @@
 // Attention over a paged cache, with or without a prefix that the whole batch
-// shares: o = sum_c e^(s_c - m) v_c / sum_c e^(s_c - m), s_c = scale q.k_c, m the
-// running maximum.
+// shares: o = sum_c e^(s_c - m) v_c / sum_c e^(s_c - m), s_c = scale q.k_c, in one
+// pass over the keys with the running maximum m.
 //
-// One wavefront per (token, head), a lane holding dim / 64 consecutive
-// elements of q, k, v and o; one pass over the keys.
+// The query heads of one kv head see the same keys, so a sequence's rows are
+// its (token, head of the group) pairs, `group` to a token.  A work item is
+// (kv head, sixteen rows, a range of keys) on one workgroup of four wavefronts;
+// where there are fewer items than the device needs, the keys are divided and a
+// second launch merges the parts.  For the prefix the rows are those of the whole
+// batch, so that its keys are read once for sixteen rows of any sequences.
+//
+// cache_attend_kernel.  Scores are S^T = K Q^T on 16x16 MFMAs (keys on the M
+// axis): lane (j = lane % 16, g = lane / 16) ends with S[row j][key 4 g + i], i <
+// 4, which is the operand layout that the product O^T += V^T P^T takes its weights
+// in, so they never change lanes.  Every wavefront streams keys of its own
+// (tiles of 32 keys in 16 bits, 16 in 32): K from memory straight into the MFMA
+// operand, a lane 16 bytes of its key's row; V in whole rows into registers,
+// which are refilled as soon as their tile is used, so that 16 KiB of a
+// wavefront (dim 128) are always under way, without a barrier.  In 16 bits V
+// goes through a tile of LDS of the wavefront's own to be read transposed
+// (ds_read_b64_tr_b16: in a 16-lane group, lane i receives element i % 4 of the
+// 8-byte pieces that lanes 4 e + i / 4 read); in 32 bits a lane's 16 bytes are
+// one element each of four MFMA operands, whose columns are dealt accordingly.
+// At dim 768 the four wavefronts share their keys and own 192 columns each; the
+// shares of the scores are summed through LDS, one barrier a tile.
+//
+// Keys beyond the last row's reach are read from the last key within it, so that
+// nothing is read that no row sees; keys that some rows of a tile do not see get
+// the weight zero, and if such a tile's V holds infinities or NaN its
+// product is formed row by row without them (0 * inf would be NaN).
+#include <algorithm>
+
 #include "xattn_cache.h"
 #include "xattn_launch.h"
 
 namespace xattn {
 namespace cache {
 
-template <typename T, int E>
-struct alignas(sizeof(T) * (E & -E)) Part {
-    T e[E];
+constexpr int kRows = 16;  // rows of a work item
+constexpr int kWaves = 4;
+
+struct AttendParams {
+    Pages pages;
+    Batch batch;
+    const int* prefix_pages;
+    int prefix_len, heads;
+    FastDiv group;
+    const void* q;
+    void* out;
+    long long qs, os;
+    float c2;         // scale * log2(e): scores in base-2 exponents
+    int causal;
+    int tiles;        // row tiles of a (kv head, range), at most
+    int single;       // every sequence has one row tile: tile b is sequence b
+    int splits, chunk;  // ranges of keys; split s holds [s * chunk, ...), the last one the rest
+    int slot, slots;  // first part of a row that this launch writes, parts of a row
+    float* po;        // [token][head][slots][dim] unnormalised
+    float2* ml;       // [token][head][slots] (maximum, sum)
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void cache_attend_kernel(Attention a) {
-    constexpr int E = D / kWave;
-    typedef Part<T, E> P;
-    const int lane = threadIdx.x % kWave;
-    const long long item = (long long)blockIdx.x * 4 + threadIdx.x / kWave;
-    const int t = (int)(item / a.heads), h = (int)(item - (long long)t * a.heads);
-    if (t >= a.batch.tokens) return;
-    const int b = token_sequence(a.batch, t);
-    if (b >= a.batch.batch) return;
-    int first, end;
-    sequence_rows(a.batch, b, &first, &end);
-    if (t < first || t >= end) return;
-    const long long len = a.batch.kv_lens[b];
-    bool bad = len < 0 || len > a.batch.capacity;
-    long long seen = len;
-    if (a.causal) seen = len - (a.batch.q_starts[b + 1] - t) + 1;
-    const unsigned kvh = h / (a.heads / a.pages.kv_heads), ps = a.pages.page_size.d;
-    const P qp = *(const P*)((const T*)a.q + t * a.qs + (long long)h * D + lane * E);
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
-    for (int e = 0; e < E; ++e) q[e] = to_f32(qp.e[e]) * a.scale * kLog2e, o[e] = 0.0f;
-    for (int part = 0; part < 2; ++part) {
-        const long long n = part ? (bad ? 0 : seen) : a.prefix_len;
-        const int* table = part ? a.batch.page_table + (long long)b * a.batch.width : a.prefix_pages;
-        for (long long c = 0; c < n; ++c) {
-            const unsigned page = a.pages.page_size.div((unsigned)c);
-            const int id = table[page];
-            if (id < 0 || (unsigned)id >= a.pages.num_pages) {
-                bad = true;
-                break;
-            }
-            const size_t row = ((size_t)id * a.pages.kv_heads + kvh) * ps + ((unsigned)c - page * ps);
-            const P kp = *(const P*)((const T*)a.pages.k + row * D + lane * E);
-            const P vp = *(const P*)((const T*)a.pages.v + row * D + lane * E);
-            float s = 0.0f;
-            for (int e = 0; e < E; ++e) s += q[e] * to_f32(kp.e[e]);
-            s = wave_sum(s);
-            const float to = fmaxf(m, s);
-            const float keep = m == to ? 1.0f : fast_exp2(m - to), w = fast_exp2(s - to);
-            m = to;
-            l = l * keep + w;
-            for (int e = 0; e < E; ++e) o[e] = o[e] * keep + w * to_f32(vp.e[e]);
-        }
-    }
-    const bool any = a.prefix_len > 0 || seen > 0;
-    P out;
-    for (int e = 0; e < E; ++e)
-        out.e[e] = from_f32<T>(bad ? NAN : any ? o[e] / l : 0.0f);
-    *(P*)((T*)a.out + t * a.os + (long long)h * D + lane * E) = out;
-}
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
 
-size_t attention_scratch(const Attention&) { return 0; }
+template <typename T> struct Vec8;
+template <> struct Vec8<_Float16> { typedef h8 type; };
+template <> struct Vec8<__bf16> { typedef bf8 type; };
+template <> struct Vec8<float> { typedef f4 type; };  // not used
 
 template <typename T>
-static void go(const Attention& a, hipStream_t stream) {
-    const unsigned grid = (unsigned)(((long long)a.batch.tokens * a.heads + 3) / 4);
-    if (a.pages.dim == 64) cache_attend_kernel<T, 64><<<grid, 256, 0, stream>>>(a);
-    if (a.pages.dim == 128) cache_attend_kernel<T, 128><<<grid, 256, 0, stream>>>(a);
-    if (a.pages.dim == 256) cache_attend_kernel<T, 256><<<grid, 256, 0, stream>>>(a);
-    if (a.pages.dim == 768) cache_attend_kernel<T, 768><<<grid, 256, 0, stream>>>(a);
+__device__ inline f4 mfma32(u4 a, u4 b, f4 c) {
+    typedef typename Vec8<T>::type V;
+    if constexpr (__is_same(T, _Float16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a),
+                                                      __builtin_bit_cast(V, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a),
+                                                       __builtin_bit_cast(V, b), c, 0, 0, 0);
+}
+__device__ inline f4 mfma4(float a, float b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-bool launch_attention(const Attention& a, void*, hipStream_t stream) {
-    if (a.dtype == XATTN_F32) go<float>(a, stream);
-    if (a.dtype == XATTN_F16) go<_Float16>(a, stream);
-    if (a.dtype == XATTN_BF16) go<__bf16>(a, stream);
+template <typename T>
+__device__ inline unsigned pack2(float lo, float hi) {
+    const T a = (T)lo, b = (T)hi;
+    return (unsigned)__builtin_bit_cast(u16, a) | (unsigned)__builtin_bit_cast(u16, b) << 16;
+}
+
+// A register of elements holds one that is infinite or NaN.
+template <typename T>
+__device__ inline bool not_finite(unsigned x) {
+    if constexpr (sizeof(T) == 4) return (x & 0x7f800000u) == 0x7f800000u;
+    constexpr unsigned e = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+    return (x & e) == e || (x >> 16 & e) == e;
+}
+
+// A sequence as an item sees it.
+struct Sequence {
+    int first, end;  // token rows
+    int len;         // keys; 0 where it is bad
+    bool bad;        // a length that its row of page_table cannot hold
+    // Keys that token row t sees.
+    __device__ int seen(int t, bool causal) const {
+        if (!causal) return len;
+        const long long n = (long long)len - (last - t) + 1;
+        return n < 0 ? 0 : n < len ? (int)n : len;
+    }
+    int last;        // q_starts[b + 1], as it is given
+};
+
+__device__ inline Sequence sequence(const Batch& B, int b) {
+    Sequence s;
+    sequence_rows(B, b, &s.first, &s.end);
+    s.last = B.q_starts[b + 1];
+    s.len = B.kv_lens[b];
+    s.bad = s.len < 0 || s.len > B.capacity;
+    if (s.bad) s.len = 0;
+    return s;
+}
+
+// The sequence that row tile `tile` of the batch lies in and its place there,
+// last tile first (under a causal mask it has the most keys).  False: none.
+__device__ inline bool find_tile(const Batch& B, int group, int tile, int* seq, int* local) {
+    const int lane = threadIdx.x % kWave;
+    for (int at = 0; at < B.batch; at += kWave) {
+        int n = 0;
+        if (at + lane < B.batch) {
+            int first, end;
+            sequence_rows(B, at + lane, &first, &end);
+            n = end > first ? (int)(((long long)(end - first) * group + kRows - 1) / kRows) : 0;
+        }
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < kWave; o *= 2) {
+            const int below = __shfl_up(sum, o);
+            if (lane >= o) sum += below;
+        }
+        const unsigned long long past = __ballot(sum > tile);
+        if (past) {
+            const int l = __ffsll(past) - 1;
+            *seq = at + l;
+            *local = __shfl(sum, l) - 1 - tile;
+            return true;
+        }
+        tile -= __shfl(sum, kWave - 1);
+    }
+    return false;
+}
+
+template <typename T, int D>
+struct Shape {
+    static constexpr bool kWide = sizeof(T) == 4;
+    static constexpr int kCols = D > 256 ? kWaves : 1;  // wavefronts that share a tile's columns
+    static constexpr int kDW = D / kCols;               // columns of a wavefront
+    static constexpr int kKeys = kWide ? 16 : 32;       // keys of a tile
+    static constexpr int kRegs = kDW / 16;              // 16-byte registers of a lane for K, for V
+    static constexpr int kBlocks = kDW / 16;            // 16-column blocks of the output
+    static constexpr int kPieces = kDW * (int)sizeof(T) / 16;  // of a row's columns
+    static constexpr int kVRow = kDW * 2 + 32;          // bytes of a V row in LDS: 32 of padding
+                                                        // deal four rows to distinct banks
+    static constexpr int kVTile = kWide ? 0 : kKeys * kVRow;
+    static constexpr int kORow = kDW + 4;               // floats of an output row in LDS
+    static constexpr int kWaveLds =
+        kCols > 1 ? kVTile : (kVTile > kRows * kORow * 4 ? kVTile : kRows * kORow * 4);
+    static constexpr int kShare = kKeys * kRows * 4;    // bytes of a wavefront's share of scores
+    static constexpr int kLds = kWaves * kWaveLds + (kCols > 1 ? 2 * kWaves * kShare : 0);
+};
+
+template <typename T, int D, bool PREFIX>
+__global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
+    typedef Shape<T, D> S;
+    constexpr int KT = S::kKeys, DW = S::kDW, NR = S::kRegs, NB = S::kBlocks;
+    constexpr bool WIDE = S::kWide, SHARED = S::kCols > 1;
+    __shared__ __align__(16) char lds[S::kLds];
+    __shared__ float2 stats[kWaves][kRows];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int j = lane % 16, g = lane / 16;
+    const int group = (int)p.group.d;
+
+    // The item: kv heads fastest, so that one head's items meet on one XCD when
+    // their number is a multiple of eight; key ranges slowest.
+    const unsigned kv_head = blockIdx.x % p.pages.kv_heads;
+    const unsigned rest = blockIdx.x / p.pages.kv_heads;
+    const int tile = (int)(rest % p.tiles), split = (int)(rest / p.tiles);
+    Sequence s;
+    const int* table;
+    int local;
+    if constexpr (PREFIX) {
+        int hi;
+        sequence_rows(p.batch, 0, &s.first, &hi);
+        sequence_rows(p.batch, p.batch.batch - 1, &hi, &s.end);
+        s.len = p.prefix_len;
+        s.last = 0;
+        s.bad = false;
+        local = tile;
+        table = p.prefix_pages;
+    } else {
+        int b = tile;
+        local = 0;
+        if (!p.single && !find_tile(p.batch, group, tile, &b, &local)) return;
+        s = sequence(p.batch, b);
+        table = p.batch.page_table + (long long)b * p.batch.width;
+    }
+    const long long all_rows = (long long)(s.end - s.first) * group;
+    const long long row0 = (long long)local * kRows;
+    if (row0 >= all_rows) return;
+    const int rows = (int)min((long long)kRows, all_rows - row0);
+    const bool causal = !PREFIX && p.causal;
+
+    // Lane j's row.  Rows behind the last repeat it and are not stored.
+    const unsigned my_row = (unsigned)row0 + min(j, rows - 1);
+    const int my_tok = s.first + (int)p.group.div(my_row);
+    const int my_head = (int)kv_head * group + (int)(my_row - p.group.div(my_row) * group);
+    const int seen = s.seen(my_tok, causal);
+    // Reach of the first row and of the last one: the least and the most.
+    const int least = s.seen(s.first + (int)p.group.div((unsigned)row0), causal);
+    const int most = s.seen(s.first + (int)p.group.div((unsigned)row0 + rows - 1), causal);
+    const int k0 = split * p.chunk;
+    const int k1 = split == p.splits - 1 ? most : min(most, k0 + p.chunk);
+    // Without keys only the first range has anything to store (a row that sees
+    // nothing, or all of a bad sequence), and not if a merge follows.
+    if (k1 <= k0 && (split > 0 || PREFIX)) return;
+
+    const int col0 = SHARED ? wave * DW : 0;
+    u4 qr[NR];
+    {
+        const T* q = (const T*)p.q + my_tok * p.qs + (long long)my_head * D + col0;
+#pragma unroll
+        for (int r = 0; r < NR / (WIDE ? 1 : 2); ++r)
+            qr[r] = WIDE ? *(const u4*)(q + 16 * r + 4 * g) : *(const u4*)(q + 32 * r + 8 * g);
+    }
+
+    f4 o[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[b] = f4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    bool bad = false;
+
+    // Rows of the cache that a tile's keys lie on: lane's key is k + lane % KT.
+    struct Where {
+        int id;
+        unsigned slot;
+    };
+    const auto find = [&](int k) {
+        const unsigned key = (unsigned)min(k + lane % KT, k1 - 1);
+        const unsigned page = p.pages.page_size.div(key);
+        return Where{table[page], key - page * p.pages.page_size.d};
+    };
+    const auto row_of = [&](const Where& w) {
+        const bool ok = w.id >= 0 && (unsigned)w.id < p.pages.num_pages;
+        bad |= !ok;
+        return ((ok ? (unsigned)w.id : 0u) * p.pages.kv_heads + kv_head) * p.pages.page_size.d +
+               w.slot;
+    };
+    u4 kr[NR], vr[NR];
+    const auto load_k = [&](unsigned row) {
+        if constexpr (WIDE) {
+            const char* a = p.pages.k + ((size_t)__shfl(row, j) * D + col0) * 4 + 16 * g;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) kr[r] = *(const u4*)(a + 64 * r);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const char* a =
+                    p.pages.k + ((size_t)__shfl(row, 16 * h + j) * D + col0) * 2 + 16 * g;
+#pragma unroll
+                for (int r = 0; r < NR / 2; ++r) kr[h * NR / 2 + r] = *(const u4*)(a + 64 * r);
+            }
+        }
+    };
+    // V register r of a lane.  32 bits: row 4 g + r % 4, columns 64 (r / 4) + 4 j
+    // on.  16 bits: piece 64 r + lane of the tile in row order.
+    constexpr int PERIOD = 64 % S::kPieces == 0 ? 1 : S::kPieces / 8;  // registers that end a row
+    constexpr int STEP = 64 * PERIOD / S::kPieces;  // ... and the rows they hold
+    const auto v_row = [&](int r) {
+        return STEP * (r / PERIOD) + ((r % PERIOD) * 64 + lane) / S::kPieces;
+    };
+    const auto v_piece = [&](int r) { return ((r % PERIOD) * 64 + lane) % S::kPieces; };
+    const auto load_v = [&](unsigned row) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            if constexpr (WIDE)
+                vr[r] = *(const u4*)(p.pages.v +
+                                     ((size_t)__shfl(row, 4 * g + r % 4) * D + col0) * 4 +
+                                     256 * (r / 4) + 16 * j);
+            else
+                vr[r] = *(const u4*)(p.pages.v + ((size_t)__shfl(row, v_row(r)) * D + col0) * 2 +
+                                     16 * v_piece(r));
+        }
+    };
+
+    char* vt = lds + wave * S::kWaveLds;
+    const int step = SHARED ? KT : kWaves * KT;
+    int k = k0 + (SHARED ? 0 : wave * KT);
+    if (k < k1) {
+        Where next = find(k);
+        const unsigned row = row_of(next);
+        next = find(k + step);
+        load_k(row);
+        load_v(row);
+        int turn = 0;
+        for (; k < k1; k += step) {
+            const bool more = k + step < k1;
+            const Where after = find(k + 2 * step);
+            // scores
+            f4 sc[KT / 16];
+#pragma unroll
+            for (int h = 0; h < KT / 16; ++h) sc[h] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sc[0] = mfma4(__uint_as_float(kr[r][e]), __uint_as_float(qr[r][e]), sc[0]);
+                } else {
+                    const int h = r % 2, i = r / 2;
+                    sc[h] = mfma32<T>(kr[h * NR / 2 + i], qr[i], sc[h]);
+                }
+            }
+            unsigned next_row = 0;
+            if (more) {
+                next_row = row_of(next);
+                load_k(next_row);
+            }
+            next = after;
+            if constexpr (SHARED) {
+                char* share = lds + kWaves * S::kWaveLds + (turn & 1) * kWaves * S::kShare;
+                turn ^= 1;
+#pragma unroll
+                for (int h = 0; h < KT / 16; ++h)
+                    *(f4*)(share + wave * S::kShare + (h * kWave + lane) * 16) = sc[h];
+                lds_barrier();
+#pragma unroll
+                for (int h = 0; h < KT / 16; ++h) {
+                    sc[h] = *(f4*)(share + (h * kWave + lane) * 16);
+#pragma unroll
+                    for (int w = 1; w < kWaves; ++w)
+                        sc[h] += *(f4*)(share + w * S::kShare + (h * kWave + lane) * 16);
+                }
+            }
+            // softmax
+            const bool partial = k + KT > least;  // some row does not see all of the tile
+            float top = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < KT / 16; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = sc[h][i] * p.c2;
+                    if (partial && k + 16 * h + 4 * g + i >= min(seen, k1)) x = -INFINITY;
+                    sc[h][i] = x;
+                    top = fmaxf(top, x);
+                }
+            top = fmaxf(m, wave_max16_groups(top));
+            // exponents are taken from 0 while a row has seen nothing
+            const float ref = top == -INFINITY ? 0.0f : top;
+            if (__ballot(top != m)) {
+                const float keep = fast_exp2(m - ref);
+                l *= keep;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) o[b] *= keep;
+                m = top;
+            }
+#pragma unroll
+            for (int h = 0; h < KT / 16; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[h][i] = fast_exp2(sc[h][i] - ref);
+                    l += sc[h][i];
+                }
+            // product with V
+            bool odd = false;
+            if (partial) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd |= not_finite<T>(vr[r][e]);
+                odd = __ballot(odd) != 0;
+            }
+            if constexpr (WIDE) {
+                if (!odd) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o[r / 4 * 4 + e] = mfma4(__uint_as_float(vr[r][e]), sc[0][r % 4],
+                                                     o[r / 4 * 4 + e]);
+                } else {
+                    // key c of the tile: its values are in the lanes of group c / 4
+                    for (int c = 0; c < KT; ++c) {
+                        const float w = __shfl(c % 4 == 0   ? sc[0][0]
+                                               : c % 4 == 1 ? sc[0][1]
+                                               : c % 4 == 2 ? sc[0][2]
+                                                            : sc[0][3],
+                                               c / 4 * 16 + j);
+                        const bool sees = k + c < min(seen, k1);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                // column 64 (b / 4) + 4 (4 g + i) + b % 4
+                                float x = 0.0f;
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    if (c % 4 == r) x = __uint_as_float(vr[b / 4 * 4 + r][b % 4]);
+                                x = __shfl(x, c / 4 * 16 + 4 * g + i);
+                                if (sees) o[b][i] += w * x;
+                            }
+                    }
+                }
+                if (more) load_v(next_row);
+            } else {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+                    *(u4*)(vt + v_row(r) * S::kVRow + 16 * v_piece(r)) = vr[r];
+                if (more) load_v(next_row);
+                if (!odd) {
+                    const u4 w = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]),
+                                  pack2<T>(sc[1][0], sc[1][1]), pack2<T>(sc[1][2], sc[1][3])};
+                    lds_s4* at = (lds_s4*)(vt + (4 * g + j / 4) * S::kVRow + j % 4 * 8);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + 4 * b);
+                        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            at + 4 * b + 16 * S::kVRow / 8);
+                        const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                        o[b] = mfma32<T>(__builtin_bit_cast(u4, both), w, o[b]);
+                    }
+                } else {
+                    for (int c = 0; c < KT; ++c) {
+                        const f4 x = c < 16 ? sc[0] : sc[1];
+                        const float w = to_f32((T)__shfl(c % 4 == 0   ? x[0]
+                                                         : c % 4 == 1 ? x[1]
+                                                         : c % 4 == 2 ? x[2]
+                                                                      : x[3],
+                                                         c % 16 / 4 * 16 + j));
+                        const bool sees = k + c < min(seen, k1);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float v = to_f32(
+                                    *(const T*)(vt + c * S::kVRow + (16 * b + 4 * g + i) * 2));
+                                if (sees) o[b][i] += w * v;
+                            }
+                    }
+                }
+            }
+        }
+    }
+    l = wave_sum16_groups(l);
+    if (__ballot(bad)) l = NAN;
+
+    // Join the wavefronts' parts (of one maximum where they share their keys).
+    if (lane < 16) stats[wave][lane] = {m, l};
+    if constexpr (!SHARED) {
+        float* mine = (float*)vt + j * S::kORow;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if constexpr (WIDE) {
+                // blocks 4 q .. 4 q + 3 hold neighbouring columns
+                if (b % 4 == 0)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *(f4*)(mine + 16 * b + 16 * g + 4 * i) =
+                            f4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]};
+            } else {
+                *(f4*)(mine + 16 * b + 4 * g) = o[b];
+            }
+        }
+    }
+    __syncthreads();
+    const auto store = [&](int row, int col, f4 x, float mx, float sum) {
+        const unsigned r = (unsigned)row0 + row;
+        const int tok = s.first + (int)p.group.div(r);
+        const int head = (int)kv_head * group + (int)(r - p.group.div(r) * group);
+        const int n = s.seen(tok, causal);
+        const bool direct = !PREFIX && p.slot == 0 && (p.splits == 1 || n <= p.chunk);
+        if (direct) {
+            if (split > 0) return;
+            Piece4<T> y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                y.e[e] = (T)(s.bad ? NAN : n > 0 ? x[e] / sum : 0.0f);
+            *(Piece4<T>*)((T*)p.out + tok * p.os + (long long)head * D + col) = y;
+        } else if (k0 < n) {
+            const size_t at =
+                ((size_t)tok * p.heads + head) * p.slots + p.slot + split;
+            *(f4*)(p.po + at * D + col) = x;
+            if (col == 0) p.ml[at] = {mx, sum};
+        }
+    };
+    if constexpr (SHARED) {
+        if (j < rows)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if constexpr (WIDE) {
+                    if (b % 4 == 0)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            store(j, col0 + 16 * b + 16 * g + 4 * i,
+                                  f4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]}, m, l);
+                } else {
+                    store(j, col0 + 16 * b + 4 * g, o[b], m, l);
+                }
+            }
+    } else {
+        for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+            const int row = i / (D / 4), col = i % (D / 4) * 4;
+            float mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, stats[w][row].x);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+            f4 x = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float keep = fast_exp2(stats[w][row].x - ref);
+                sum += keep * stats[w][row].y;
+                x += keep * *(const f4*)((const float*)(lds + w * S::kWaveLds) + row * S::kORow +
+                                         col);
+            }
+            store(row, col, x, mx, sum);
+        }
+    }
+}
+
+// --------------------------------------------------------------------------
+// cache_merge_kernel: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the
+// parts of a row, in their order.  A workgroup takes a row; D / 4 threads hold
+// its columns, as many groups of them as fit take every so many-th part.
+// --------------------------------------------------------------------------
+constexpr int kMaxSlots = 512;
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cache_merge_kernel(AttendParams p, int prefix_splits) {
+    constexpr int TC = D / 4, GROUPS = 256 / TC;
+    __shared__ float weight[kMaxSlots];
+    __shared__ f4 sums[GROUPS > 1 ? 256 : 1];
+    __shared__ float total[2];
+    const int t = (int)(blockIdx.x / p.heads), head = (int)(blockIdx.x % p.heads);
+    const int b = token_sequence(p.batch, t);
+    if (b >= p.batch.batch) return;
+    const Sequence s = sequence(p.batch, b);
+    if (t < s.first || t >= s.end) return;
+    const int n = s.seen(t, p.causal);
+    if (p.slot == 0 && (p.splits == 1 || n <= p.chunk)) return;  // stored already
+    int own = (n + p.chunk - 1) / p.chunk;
+    if (own > p.splits) own = p.splits;
+    const int parts = prefix_splits + own;
+    const size_t at = ((size_t)t * p.heads + head) * p.slots;
+    if (threadIdx.x < kWave) {
+        float top = -INFINITY, sum = 0.0f;
+        for (int i = threadIdx.x; i < parts; i += kWave) top = fmaxf(top, p.ml[at + i].x);
+        top = wave_max(top);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        for (int i = threadIdx.x; i < parts; i += kWave) {
+            const float2 ml = p.ml[at + i];
+            weight[i] = fast_exp2(ml.x - ref);
+            sum += weight[i] * ml.y;
+        }
+        sum = wave_sum(sum);
+        if (threadIdx.x == 0) total[0] = s.bad ? NAN : sum;
+    }
+    __syncthreads();
+    const int c = threadIdx.x % TC, grp = threadIdx.x / TC;
+    f4 x = {0, 0, 0, 0};
+    if (grp < GROUPS)
+#pragma unroll 4
+        for (int i = grp; i < parts; i += GROUPS)
+            x += weight[i] * *(const f4*)(p.po + (at + i) * D + 4 * c);
+    if constexpr (GROUPS > 1) {
+        sums[threadIdx.x] = x;
+        __syncthreads();
+        if (grp > 0) return;
+#pragma unroll
+        for (int i = 1; i < GROUPS; ++i) x += sums[i * TC + c];
+    }
+    if (grp > 0) return;
+    Piece4<T> y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y.e[e] = (T)(x[e] / total[0]);
+    *(Piece4<T>*)((T*)p.out + t * p.os + (long long)head * D + 4 * c) = y;
+}
+
+// --------------------------------------------------------------------------
+// Plan
+// --------------------------------------------------------------------------
+struct Range {
+    int splits, chunk;
+};
+
+// Ranges that `keys` keys are divided into where there are `items` items of all
+// of them: enough for `want` workgroups, each at least a tile of every
+// wavefront.
+static Range ranges(long long items, int keys, int step, int most) {
+    const long long want = 4LL * device_cu_count();
+    long long s = items > 0 ? want / items : 1;
+    s = std::min<long long>(s, keys / step);
+    s = std::max<long long>(1, std::min<long long>(s, most));
+    long long chunk = (keys + s - 1) / s;
+    chunk = std::max<long long>(step, (chunk + step - 1) / step * step);
+    return {(int)std::max<long long>(1, (keys + chunk - 1) / chunk), (int)chunk};
+}
+
+struct Plan {
+    bool single;
+    int tiles, prefix_tiles;
+    Range own, prefix;
+    int prefix_splits() const { return prefix.splits; }
+    int slots() const { return own.splits + prefix.splits; }
+};
+
+static Plan plan(const Attention& a) {
+    Plan p;
+    const int kv = (int)a.pages.kv_heads, group = a.heads / kv;
+    const int step = (a.dtype == XATTN_F32 ? 16 : 32) * (a.pages.dim > 256 ? 1 : kWaves);
+    const long long rows = (long long)a.batch.tokens * group;
+    p.single = (long long)a.max_q * group <= kRows;
+    p.tiles = p.single ? a.batch.batch
+                       : (int)std::min<long long>(rows / kRows + a.batch.batch,
+                                                  ((long long)a.max_q * group + kRows - 1) /
+                                                      kRows * a.batch.batch);
+    p.own = ranges((long long)p.tiles * kv, a.max_kv, step, kMaxSlots / 2);
+    p.prefix_tiles = (int)((rows + kRows - 1) / kRows);
+    p.prefix = a.prefix_len > 0
+                   ? ranges((long long)p.prefix_tiles * kv, a.prefix_len, step, kMaxSlots / 2)
+                   : Range{0, 1};
+    return p;
+}
+
+static size_t parts(const Attention& a, const Plan& p) {
+    if (p.prefix.splits == 0 && p.own.splits == 1) return 0;
+    return (size_t)a.batch.tokens * a.heads * p.slots();
+}
+
+size_t attention_scratch(const Attention& a) {
+    return parts(a, plan(a)) * (a.pages.dim * sizeof(float) + sizeof(float2));
+}
+
+template <typename T, int D>
+static void go(AttendParams& p, const Plan& plan, hipStream_t stream) {
+    const unsigned kv = p.pages.kv_heads;
+    if (plan.prefix.splits > 0) {
+        AttendParams f = p;
+        f.tiles = plan.prefix_tiles;
+        f.splits = plan.prefix.splits;
+        f.chunk = plan.prefix.chunk;
+        f.slot = 0;
+        cache_attend_kernel<T, D, true>
+            <<<kv * plan.prefix_tiles * plan.prefix.splits, 256, 0, stream>>>(f);
+    }
+    cache_attend_kernel<T, D, false>
+        <<<kv * plan.tiles * plan.own.splits, 256, 0, stream>>>(p);
+    if (p.po)
+        cache_merge_kernel<T, D><<<(unsigned)p.batch.tokens * p.heads, 256, 0, stream>>>(
+            p, plan.prefix.splits);
+}
+
+template <typename T>
+static void by_dim(AttendParams& p, const Plan& plan, hipStream_t stream) {
+    if (p.pages.dim == 64) go<T, 64>(p, plan, stream);
+    if (p.pages.dim == 128) go<T, 128>(p, plan, stream);
+    if (p.pages.dim == 256) go<T, 256>(p, plan, stream);
+    if (p.pages.dim == kDim) go<T, kDim>(p, plan, stream);
+}
+
+bool launch_attention(const Attention& a, void* scratch, hipStream_t stream) {
+    const Plan pl = plan(a);
+    AttendParams p{};
+    p.pages = a.pages;
+    p.batch = a.batch;
+    p.prefix_pages = a.prefix_pages;
+    p.prefix_len = a.prefix_len;
+    p.heads = a.heads;
+    p.group = FastDiv::of((unsigned)a.heads / a.pages.kv_heads);
+    p.q = a.q;
+    p.out = a.out;
+    p.qs = a.qs;
+    p.os = a.os;
+    p.c2 = a.scale * kLog2e;
+    p.causal = a.causal;
+    p.tiles = pl.tiles;
+    p.single = pl.single;
+    p.splits = pl.own.splits;
+    p.chunk = pl.own.chunk;
+    p.slot = pl.prefix.splits;
+    p.slots = pl.slots();
+    if (const size_t n = parts(a, pl)) {
+        p.po = (float*)scratch;
+        p.ml = (float2*)(p.po + n * a.pages.dim);
+    }
+    if (a.dtype == XATTN_F32) by_dim<float>(p, pl, stream);
+    if (a.dtype == XATTN_F16) by_dim<_Float16>(p, pl, stream);
+    if (a.dtype == XATTN_BF16) by_dim<__bf16>(p, pl, stream);
     return check_launch("cache_attend_kernel");
 }
 

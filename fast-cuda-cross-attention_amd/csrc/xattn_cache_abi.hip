@@ -130,7 +130,7 @@ static bool view_attention(const char* who, const xattn_kv_cache* cache, const x
                   cache->kv_heads);
         return false;
     }
-    if ((long long)heads * std::max(batch->tokens, 1) > 0x7fffffLL * 64) {
+    if ((long long)heads * std::max(std::max(batch->tokens, batch->batch), 1) > 0x1fffffff) {
         set_error(XATTN_ERR_UNSUPPORTED, "%s: %d tokens of %d heads in one call", who,
                   batch->tokens, heads);
         return false;
