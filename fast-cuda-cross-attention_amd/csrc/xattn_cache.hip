@@ -26,8 +26,7 @@
 //
 // Keys beyond the last row's reach are read from the last key within it, so that
 // nothing is read that no row sees; keys that some rows of a tile do not see get
-// the weight zero, and if such a tile's V holds infinities or NaN its
-// product is formed row by row without them (0 * inf would be NaN).
+// the weight zero there.
 #include <algorithm>
 
 #include "xattn_cache.h"
@@ -36,7 +35,8 @@
 namespace xattn {
 namespace cache {
 
-constexpr int kRows = 16;  // rows of a work item
+constexpr int kRows = 16;      // rows of a work item of cache_attend_kernel
+constexpr int kManyRows = 32;  // rows beyond which cache_tile_kernel takes over
 constexpr int kWaves = 4;
 
 struct AttendParams {
@@ -59,6 +59,7 @@ struct AttendParams {
 };
 
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
@@ -87,12 +88,40 @@ __device__ inline unsigned pack2(float lo, float hi) {
     return (unsigned)__builtin_bit_cast(u16, a) | (unsigned)__builtin_bit_cast(u16, b) << 16;
 }
 
-// A register of elements holds one that is infinite or NaN.
+// Infinities and NaN in V.  A weight of zero does not silence them in a matrix
+// product (0 * inf is NaN), so in tiles that some rows do not see all of they
+// are cleared before it; if there were any, those keys are gone through once
+// more at the end, and added to the rows that see them as they are: a
+// weight is positive, and no finite sum changes what they make of it.
 template <typename T>
-__device__ inline bool not_finite(unsigned x) {
-    if constexpr (sizeof(T) == 4) return (x & 0x7f800000u) == 0x7f800000u;
-    constexpr unsigned e = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
-    return (x & e) == e || (x >> 16 & e) == e;
+__device__ inline bool clear_not_finite(u4& x) {
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 4) {
+            const bool is = (x[e] & 0x7f800000u) == 0x7f800000u;
+            any |= is;
+            if (is) x[e] = 0;
+        } else {
+            constexpr unsigned m = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+            const bool lo = (x[e] & m) == m, hi = (x[e] >> 16 & m) == m;
+            any |= lo | hi;
+            x[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+        }
+    }
+    return any;
+}
+// Four elements of V with all but infinities and NaN cleared.
+template <typename T>
+__device__ inline f4 odd_values(const char* v) {
+    const Piece4<T> x = *(const Piece4<T>*)v;
+    f4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float f = to_f32(x.e[e]);
+        y[e] = __builtin_isfinite(f) ? 0.0f : f;
+    }
+    return y;
 }
 
 // A sequence as an item sees it.
@@ -121,6 +150,7 @@ __device__ inline Sequence sequence(const Batch& B, int b) {
 
 // The sequence that row tile `tile` of the batch lies in and its place there,
 // last tile first (under a causal mask it has the most keys).  False: none.
+template <int ROWS>
 __device__ inline bool find_tile(const Batch& B, int group, int tile, int* seq, int* local) {
     const int lane = threadIdx.x % kWave;
     for (int at = 0; at < B.batch; at += kWave) {
@@ -128,7 +158,7 @@ __device__ inline bool find_tile(const Batch& B, int group, int tile, int* seq, 
         if (at + lane < B.batch) {
             int first, end;
             sequence_rows(B, at + lane, &first, &end);
-            n = end > first ? (int)(((long long)(end - first) * group + kRows - 1) / kRows) : 0;
+            n = end > first ? (int)(((long long)(end - first) * group + ROWS - 1) / ROWS) : 0;
         }
         int sum = n;
 #pragma unroll
@@ -146,6 +176,107 @@ __device__ inline bool find_tile(const Batch& B, int group, int tile, int* seq, 
         tile -= __shfl(sum, kWave - 1);
     }
     return false;
+}
+
+// A work item: rows row0 .. row0 + rows - 1 of a sequence (of the whole batch
+// for the prefix) and kv head, and the keys k0 .. k1 - 1.
+struct Row {
+    int token, head;
+};
+struct Item {
+    Sequence s;
+    const int* table;
+    unsigned row0, kv_head;
+    int rows, split, k0, k1;
+    int least;  // keys that all of its rows see
+    bool causal;
+    __device__ Row row(const AttendParams& p, int i) const {
+        const unsigned r = row0 + i, t = p.group.div(r);
+        return {s.first + (int)t, (int)(kv_head * p.group.d + r - t * p.group.d)};
+    }
+    // V's row of a key within k0 .. k1 - 1, of `bytes` bytes; null on a bad page.
+    __device__ const char* row_of_v(const AttendParams& p, int k, int bytes) const {
+        const unsigned page = p.pages.page_size.div((unsigned)k), size = p.pages.page_size.d;
+        const int id = table[page];
+        if (id < 0 || (unsigned)id >= p.pages.num_pages) return nullptr;
+        return p.pages.v + (size_t)(((unsigned)id * p.pages.kv_heads + kv_head) * size +
+                                    ((unsigned)k - page * size)) * bytes;
+    }
+};
+
+// The workgroup's item; false where it has none.  Row tiles of one kv head and
+// key range read the same keys: where those streams deal evenly onto the eight
+// XCDs, all tiles of a stream go to one of them and follow each other there, so
+// that its L2 reads the keys once.  Otherwise kv heads go fastest and key
+// ranges slowest, and of a ragged batch the ranges that few sequences have come
+// last.
+template <int ROWS, bool PREFIX>
+__device__ inline bool find_item(const AttendParams& p, Item* it) {
+    unsigned tile, stream;
+    const unsigned streams = p.pages.kv_heads * p.splits;
+    if (!p.single && streams % kNumXcd == 0) {
+        const unsigned at = blockIdx.x / kNumXcd;
+        stream = blockIdx.x % kNumXcd + at / p.tiles * kNumXcd;
+        tile = at % p.tiles;
+        it->kv_head = stream % p.pages.kv_heads;
+        it->split = (int)(stream / p.pages.kv_heads);
+    } else {
+        const unsigned rest = blockIdx.x / p.pages.kv_heads;
+        it->kv_head = blockIdx.x % p.pages.kv_heads;
+        tile = rest % p.tiles;
+        it->split = (int)(rest / p.tiles);
+    }
+    int local = (int)tile;
+    if constexpr (PREFIX) {
+        int other;
+        sequence_rows(p.batch, 0, &it->s.first, &other);
+        sequence_rows(p.batch, p.batch.batch - 1, &other, &it->s.end);
+        it->s.len = p.prefix_len;
+        it->s.last = 0;
+        it->s.bad = false;
+        it->table = p.prefix_pages;
+    } else {
+        int b = (int)tile;
+        if (p.single)
+            local = 0;
+        else if (!find_tile<ROWS>(p.batch, (int)p.group.d, (int)tile, &b, &local))
+            return false;
+        it->s = sequence(p.batch, b);
+        it->table = p.batch.page_table + (long long)b * p.batch.width;
+    }
+    it->causal = !PREFIX && p.causal;
+    const long long all = (long long)(it->s.end - it->s.first) * p.group.d;
+    const long long row0 = (long long)local * ROWS;
+    if (row0 >= all) return false;
+    it->row0 = (unsigned)row0;
+    it->rows = (int)min((long long)ROWS, all - row0);
+    it->least = it->s.seen(it->row(p, 0).token, it->causal);
+    const int most = it->s.seen(it->row(p, it->rows - 1).token, it->causal);
+    it->k0 = it->split * p.chunk;
+    it->k1 = it->split == p.splits - 1 ? most : min(most, it->k0 + p.chunk);
+    // Without keys only the first range may have something to store: rows that
+    // see nothing, or those of a bad sequence.
+    return it->k1 > it->k0 || (it->split == 0 && !PREFIX);
+}
+
+// Stores four columns of a row's result: as a part (unnormalised, with its
+// maximum and sum) if a merge follows for the row, otherwise as output.
+template <typename T, int D, bool PREFIX>
+__device__ inline void store(const AttendParams& p, const Item& it, int row, int col, f4 x,
+                             float top, float sum) {
+    const Row r = it.row(p, row);
+    const int n = it.s.seen(r.token, it.causal);
+    if (!PREFIX && p.slot == 0 && (p.splits == 1 || n <= p.chunk)) {
+        if (it.split > 0) return;
+        Piece4<T> y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y.e[e] = (T)(it.s.bad ? NAN : n > 0 ? x[e] / sum : 0.0f);
+        *(Piece4<T>*)((T*)p.out + r.token * p.os + (long long)r.head * D + col) = y;
+    } else if (it.k0 < n) {
+        const size_t at = ((size_t)r.token * p.heads + r.head) * p.slots + p.slot + it.split;
+        *(f4*)(p.po + at * D + col) = x;
+        if (col == 0) p.ml[at] = {top, sum};
+    }
 }
 
 template <typename T, int D>
@@ -176,56 +307,21 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
     __shared__ float2 stats[kWaves][kRows];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int j = lane % 16, g = lane / 16;
-    const int group = (int)p.group.d;
 
-    // The item: kv heads fastest, so that one head's items meet on one XCD when
-    // their number is a multiple of eight; key ranges slowest.
-    const unsigned kv_head = blockIdx.x % p.pages.kv_heads;
-    const unsigned rest = blockIdx.x / p.pages.kv_heads;
-    const int tile = (int)(rest % p.tiles), split = (int)(rest / p.tiles);
-    Sequence s;
-    const int* table;
-    int local;
-    if constexpr (PREFIX) {
-        int hi;
-        sequence_rows(p.batch, 0, &s.first, &hi);
-        sequence_rows(p.batch, p.batch.batch - 1, &hi, &s.end);
-        s.len = p.prefix_len;
-        s.last = 0;
-        s.bad = false;
-        local = tile;
-        table = p.prefix_pages;
-    } else {
-        int b = tile;
-        local = 0;
-        if (!p.single && !find_tile(p.batch, group, tile, &b, &local)) return;
-        s = sequence(p.batch, b);
-        table = p.batch.page_table + (long long)b * p.batch.width;
-    }
-    const long long all_rows = (long long)(s.end - s.first) * group;
-    const long long row0 = (long long)local * kRows;
-    if (row0 >= all_rows) return;
-    const int rows = (int)min((long long)kRows, all_rows - row0);
-    const bool causal = !PREFIX && p.causal;
+    Item it;
+    if (!find_item<kRows, PREFIX>(p, &it)) return;
+    const Sequence& s = it.s;
+    const int rows = it.rows, least = it.least, k0 = it.k0, k1 = it.k1;
+    const unsigned kv_head = it.kv_head;
 
     // Lane j's row.  Rows behind the last repeat it and are not stored.
-    const unsigned my_row = (unsigned)row0 + min(j, rows - 1);
-    const int my_tok = s.first + (int)p.group.div(my_row);
-    const int my_head = (int)kv_head * group + (int)(my_row - p.group.div(my_row) * group);
-    const int seen = s.seen(my_tok, causal);
-    // Reach of the first row and of the last one: the least and the most.
-    const int least = s.seen(s.first + (int)p.group.div((unsigned)row0), causal);
-    const int most = s.seen(s.first + (int)p.group.div((unsigned)row0 + rows - 1), causal);
-    const int k0 = split * p.chunk;
-    const int k1 = split == p.splits - 1 ? most : min(most, k0 + p.chunk);
-    // Without keys only the first range has anything to store (a row that sees
-    // nothing, or all of a bad sequence), and not if a merge follows.
-    if (k1 <= k0 && (split > 0 || PREFIX)) return;
+    const Row mine = it.row(p, min(j, rows - 1));
+    const int seen = s.seen(mine.token, it.causal);
 
     const int col0 = SHARED ? wave * DW : 0;
     u4 qr[NR];
     {
-        const T* q = (const T*)p.q + my_tok * p.qs + (long long)my_head * D + col0;
+        const T* q = (const T*)p.q + mine.token * p.qs + (long long)mine.head * D + col0;
 #pragma unroll
         for (int r = 0; r < NR / (WIDE ? 1 : 2); ++r)
             qr[r] = WIDE ? *(const u4*)(q + 16 * r + 4 * g) : *(const u4*)(q + 32 * r + 8 * g);
@@ -235,7 +331,7 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b] = f4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
-    bool bad = false;
+    bool bad = false, odd = false;
 
     // Rows of the cache that a tile's keys lie on: lane's key is k + lane % KT.
     struct Where {
@@ -245,7 +341,7 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
     const auto find = [&](int k) {
         const unsigned key = (unsigned)min(k + lane % KT, k1 - 1);
         const unsigned page = p.pages.page_size.div(key);
-        return Where{table[page], key - page * p.pages.page_size.d};
+        return Where{it.table[page], key - page * p.pages.page_size.d};
     };
     const auto row_of = [&](const Where& w) {
         const bool ok = w.id >= 0 && (unsigned)w.id < p.pages.num_pages;
@@ -369,92 +465,63 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
                     l += sc[h][i];
                 }
             // product with V
-            bool odd = false;
-            if (partial) {
+            if (partial)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) odd |= clear_not_finite<T>(vr[r]);
+            if constexpr (WIDE) {
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) odd |= not_finite<T>(vr[r][e]);
-                odd = __ballot(odd) != 0;
-            }
-            if constexpr (WIDE) {
-                if (!odd) {
-#pragma unroll
-                    for (int r = 0; r < NR; ++r)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            o[r / 4 * 4 + e] = mfma4(__uint_as_float(vr[r][e]), sc[0][r % 4],
-                                                     o[r / 4 * 4 + e]);
-                } else {
-                    // key c of the tile: its values are in the lanes of group c / 4
-                    for (int c = 0; c < KT; ++c) {
-                        const float w = __shfl(c % 4 == 0   ? sc[0][0]
-                                               : c % 4 == 1 ? sc[0][1]
-                                               : c % 4 == 2 ? sc[0][2]
-                                                            : sc[0][3],
-                                               c / 4 * 16 + j);
-                        const bool sees = k + c < min(seen, k1);
-#pragma unroll
-                        for (int b = 0; b < NB; ++b)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                // column 64 (b / 4) + 4 (4 g + i) + b % 4
-                                float x = 0.0f;
-#pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    if (c % 4 == r) x = __uint_as_float(vr[b / 4 * 4 + r][b % 4]);
-                                x = __shfl(x, c / 4 * 16 + 4 * g + i);
-                                if (sees) o[b][i] += w * x;
-                            }
-                    }
-                }
+                    for (int e = 0; e < 4; ++e)
+                        o[r / 4 * 4 + e] =
+                            mfma4(__uint_as_float(vr[r][e]), sc[0][r % 4], o[r / 4 * 4 + e]);
                 if (more) load_v(next_row);
             } else {
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
                     *(u4*)(vt + v_row(r) * S::kVRow + 16 * v_piece(r)) = vr[r];
                 if (more) load_v(next_row);
-                if (!odd) {
-                    const u4 w = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]),
-                                  pack2<T>(sc[1][0], sc[1][1]), pack2<T>(sc[1][2], sc[1][3])};
-                    lds_s4* at = (lds_s4*)(vt + (4 * g + j / 4) * S::kVRow + j % 4 * 8);
+                const u4 w = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]),
+                              pack2<T>(sc[1][0], sc[1][1]), pack2<T>(sc[1][2], sc[1][3])};
+                lds_s4* at = (lds_s4*)(vt + (4 * g + j / 4) * S::kVRow + j % 4 * 8);
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + 4 * b);
-                        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            at + 4 * b + 16 * S::kVRow / 8);
-                        const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                        o[b] = mfma32<T>(__builtin_bit_cast(u4, both), w, o[b]);
-                    }
-                } else {
-                    for (int c = 0; c < KT; ++c) {
-                        const f4 x = c < 16 ? sc[0] : sc[1];
-                        const float w = to_f32((T)__shfl(c % 4 == 0   ? x[0]
-                                                         : c % 4 == 1 ? x[1]
-                                                         : c % 4 == 2 ? x[2]
-                                                                      : x[3],
-                                                         c % 16 / 4 * 16 + j));
-                        const bool sees = k + c < min(seen, k1);
-#pragma unroll
-                        for (int b = 0; b < NB; ++b)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float v = to_f32(
-                                    *(const T*)(vt + c * S::kVRow + (16 * b + 4 * g + i) * 2));
-                                if (sees) o[b][i] += w * v;
-                            }
-                    }
+                for (int b = 0; b < NB; ++b) {
+                    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + 4 * b);
+                    const s4 hi =
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + 4 * b + 16 * S::kVRow / 8);
+                    const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[b] = mfma32<T>(__builtin_bit_cast(u4, both), w, o[b]);
                 }
             }
         }
     }
+    if (__ballot(odd))
+        for (int t = k0 + (SHARED ? 0 : wave * KT); t < k1; t += step)
+            for (int c = t; t + KT > least && c < min(t + KT, k1); ++c)
+                if (const char* v = it.row_of_v(p, c, D * (int)sizeof(T)))
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        // 32 bits: element i of block b is column 64 (b / 4) + 16 g + 4 i + b % 4
+                        f4 x;
+                        if constexpr (WIDE) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float f = *(const float*)(
+                                    v + (col0 + 64 * (b / 4) + 16 * g + 4 * i + b % 4) * 4);
+                                x[i] = __builtin_isfinite(f) ? 0.0f : f;
+                            }
+                        } else {
+                            x = odd_values<T>(v + (col0 + 16 * b + 4 * g) * 2);
+                        }
+                        if (c < seen) o[b] += x;
+                    }
     l = wave_sum16_groups(l);
     if (__ballot(bad)) l = NAN;
 
     // Join the wavefronts' parts (of one maximum where they share their keys).
     if (lane < 16) stats[wave][lane] = {m, l};
     if constexpr (!SHARED) {
-        float* mine = (float*)vt + j * S::kORow;
+        float* part = (float*)vt + j * S::kORow;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             if constexpr (WIDE) {
@@ -462,34 +529,14 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
                 if (b % 4 == 0)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        *(f4*)(mine + 16 * b + 16 * g + 4 * i) =
+                        *(f4*)(part + 16 * b + 16 * g + 4 * i) =
                             f4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]};
             } else {
-                *(f4*)(mine + 16 * b + 4 * g) = o[b];
+                *(f4*)(part + 16 * b + 4 * g) = o[b];
             }
         }
     }
     __syncthreads();
-    const auto store = [&](int row, int col, f4 x, float mx, float sum) {
-        const unsigned r = (unsigned)row0 + row;
-        const int tok = s.first + (int)p.group.div(r);
-        const int head = (int)kv_head * group + (int)(r - p.group.div(r) * group);
-        const int n = s.seen(tok, causal);
-        const bool direct = !PREFIX && p.slot == 0 && (p.splits == 1 || n <= p.chunk);
-        if (direct) {
-            if (split > 0) return;
-            Piece4<T> y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                y.e[e] = (T)(s.bad ? NAN : n > 0 ? x[e] / sum : 0.0f);
-            *(Piece4<T>*)((T*)p.out + tok * p.os + (long long)head * D + col) = y;
-        } else if (k0 < n) {
-            const size_t at =
-                ((size_t)tok * p.heads + head) * p.slots + p.slot + split;
-            *(f4*)(p.po + at * D + col) = x;
-            if (col == 0) p.ml[at] = {mx, sum};
-        }
-    };
     if constexpr (SHARED) {
         if (j < rows)
 #pragma unroll
@@ -498,10 +545,10 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
                     if (b % 4 == 0)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            store(j, col0 + 16 * b + 16 * g + 4 * i,
+                            store<T, D, PREFIX>(p, it, j, col0 + 16 * b + 16 * g + 4 * i,
                                   f4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]}, m, l);
                 } else {
-                    store(j, col0 + 16 * b + 4 * g, o[b], m, l);
+                    store<T, D, PREFIX>(p, it, j, col0 + 16 * b + 4 * g, o[b], m, l);
                 }
             }
     } else {
@@ -519,8 +566,221 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
                 x += keep * *(const f4*)((const float*)(lds + w * S::kWaveLds) + row * S::kORow +
                                          col);
             }
-            store(row, col, x, mx, sum);
+            store<T, D, PREFIX>(p, it, row, col, x, mx, sum);
         }
+    }
+}
+
+// --------------------------------------------------------------------------
+// cache_tile_kernel: the same in 16 bits for many rows.  Each of the four
+// wavefronts holds RB blocks of sixteen rows, all share tiles of K and V in
+// LDS (two of each, filled through registers while the tile before is worked
+// on; one barrier a tile).  An operand of K or V read from LDS feeds RB matrix
+// instructions.  Weights are taken relative to a maximum that is renewed only
+// when a score exceeds it by kLag (in exponents of 2), so that the output is
+// rarely rescaled; they stay below 2^kLag, far from the range of either type.
+// --------------------------------------------------------------------------
+constexpr float kLag = 8.0f;
+
+template <int D>
+struct TileShape {
+    static constexpr int kBlocks = D > 128 ? 1 : 2;       // row blocks of a wavefront (RB)
+    static constexpr int kRows = 16 * kBlocks * kWaves;   // rows of a workgroup
+    static constexpr int kKeys = D > 128 ? 32 : 64;       // keys of a tile
+    static constexpr int kPieces = D / 8;                 // 16-byte pieces of a row
+    static constexpr int kLoads = kKeys * kPieces / 256;  // pieces of a thread, of K and of V
+    static constexpr int kLdsRow = D * 2 + 32;
+    static constexpr int kTile = kKeys * kLdsRow;
+};
+
+template <typename T, int D, bool PREFIX>
+__global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
+    typedef TileShape<D> S;
+    constexpr int RB = S::kBlocks, KT = S::kKeys, KB = KT / 16, NL = S::kLoads;
+    constexpr int DS = D / 32, DB = D / 16, LR = S::kLdsRow;
+    __shared__ __align__(16) char lds[4 * S::kTile];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int j = lane % 16, g = lane / 16;
+    Item it;
+    if (!find_item<S::kRows, PREFIX>(p, &it)) return;
+    const Sequence& s = it.s;
+    const int k0 = it.k0, k1 = it.k1;
+
+    int seen[RB];
+    u4 q[RB][DS];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const Row r = it.row(p, min(16 * (wave * RB + b) + j, it.rows - 1));
+        seen[b] = min(s.seen(r.token, it.causal), k1);
+        const T* from = (const T*)p.q + r.token * p.qs + (long long)r.head * D + 8 * g;
+#pragma unroll
+        for (int i = 0; i < DS; ++i) q[b][i] = *(const u4*)(from + 32 * i);
+    }
+    f4 o[RB][DB];
+    float m[RB], l[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        m[b] = -INFINITY;
+        l[b] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[b][i] = f4{0, 0, 0, 0};
+    }
+
+    // A thread's pieces of a tile: piece threadIdx % kPieces of every so many-th row.
+    constexpr int STRIDE = 256 / S::kPieces;
+    const int piece = threadIdx.x % S::kPieces, first = threadIdx.x / S::kPieces;
+    bool bad = false, odd = false;
+    int id[NL];
+    unsigned slot[NL];
+    const auto find = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const unsigned key = (unsigned)min(k + first + STRIDE * i, k1 - 1);
+            const unsigned page = p.pages.page_size.div(key);
+            id[i] = it.table[page];
+            slot[i] = key - page * p.pages.page_size.d;
+        }
+    };
+    u4 kr[NL], vr[NL];
+    size_t at[NL];
+    const auto load_k = [&]() {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const bool ok = id[i] >= 0 && (unsigned)id[i] < p.pages.num_pages;
+            bad |= !ok;
+            at[i] = (size_t)(((ok ? (unsigned)id[i] : 0u) * p.pages.kv_heads + it.kv_head) *
+                                 p.pages.page_size.d + slot[i]) * (D * 2) + 16 * piece;
+            kr[i] = *(const u4*)(p.pages.k + at[i]);
+        }
+    };
+    const auto load_v = [&]() {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) vr[i] = *(const u4*)(p.pages.v + at[i]);
+    };
+    char* const mine = lds + first * LR + 16 * piece;
+    const auto put_k = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            *(u4*)(mine + (t & 1) * 2 * S::kTile + i * STRIDE * LR) = kr[i];
+    };
+    const auto put_v = [&](int t, bool partial) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            if (partial) odd |= clear_not_finite<T>(vr[i]);
+            *(u4*)(mine + ((t & 1) * 2 + 1) * S::kTile + i * STRIDE * LR) = vr[i];
+        }
+    };
+
+    if (k0 < k1) {
+        find(k0);
+        load_k();
+        load_v();
+        find(k0 + KT);
+        put_k(0);
+        put_v(0, k0 + KT > it.least);
+    }
+    __syncthreads();
+    int t = 0;
+    for (int k = k0; k < k1; k += KT, ++t) {
+        const bool more = k + KT < k1;
+        if (more) {
+            load_k();
+            find(k + 2 * KT);
+        }
+        const char* kt = lds + (t & 1) * 2 * S::kTile;
+        const char* vt = kt + S::kTile;
+        f4 sc[RB][KB];
+#pragma unroll
+        for (int h = 0; h < KB; ++h) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b) sc[b][h] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < DS; ++i) {
+                const u4 a = *(const u4*)(kt + (16 * h + j) * LR + 64 * i + 16 * g);
+#pragma unroll
+                for (int b = 0; b < RB; ++b) sc[b][h] = mfma32<T>(a, q[b][i], sc[b][h]);
+            }
+        }
+        const bool partial = k + KT > it.least;
+        u4 w[RB][KB / 2];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < KB; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = sc[b][h][i] * p.c2;
+                    if (partial && k + 16 * h + 4 * g + i >= seen[b]) x = -INFINITY;
+                    sc[b][h][i] = x;
+                    top = fmaxf(top, x);
+                }
+            top = wave_max16_groups(top);
+            if (__ballot(top > m[b] + kLag)) {
+                top = fmaxf(m[b], top);
+                const float keep = top == -INFINITY ? 1.0f : fast_exp2(m[b] - top);
+                l[b] *= keep;
+#pragma unroll
+                for (int i = 0; i < DB; ++i) o[b][i] *= keep;
+                m[b] = top;
+            }
+            const float ref = m[b] == -INFINITY ? 0.0f : m[b];
+#pragma unroll
+            for (int h = 0; h < KB; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[b][h][i] = fast_exp2(sc[b][h][i] - ref);
+                    l[b] += sc[b][h][i];
+                }
+#pragma unroll
+            for (int h = 0; h < KB / 2; ++h)
+                w[b][h] = u4{pack2<T>(sc[b][2 * h][0], sc[b][2 * h][1]),
+                             pack2<T>(sc[b][2 * h][2], sc[b][2 * h][3]),
+                             pack2<T>(sc[b][2 * h + 1][0], sc[b][2 * h + 1][1]),
+                             pack2<T>(sc[b][2 * h + 1][2], sc[b][2 * h + 1][3])};
+        }
+        if (more) {
+            put_k(t + 1);
+            load_v();
+        }
+        lds_s4* from = (lds_s4*)(vt + (4 * g + j / 4) * LR + j % 4 * 8);
+#pragma unroll
+        for (int h = 0; h < KB / 2; ++h)
+#pragma unroll
+            for (int i = 0; i < DB; ++i) {
+                const s4 lo =
+                    __builtin_amdgcn_ds_read_tr16_b64_v4i16(from + 4 * i + 32 * h * LR / 8);
+                const s4 hi =
+                    __builtin_amdgcn_ds_read_tr16_b64_v4i16(from + 4 * i + (32 * h + 16) * LR / 8);
+                const u4 a = __builtin_bit_cast(
+                    u4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int b = 0; b < RB; ++b) o[b][i] = mfma32<T>(a, w[b][h], o[b][i]);
+            }
+        if (more) put_v(t + 1, k + 2 * KT > it.least);
+        lds_barrier();
+    }
+    if (__syncthreads_or(bad))
+#pragma unroll
+        for (int b = 0; b < RB; ++b) l[b] = NAN;
+    if (__syncthreads_or(odd))
+        for (int k = max(k0, it.least / KT * KT); k < k1; ++k)
+            if (const char* v = it.row_of_v(p, k, D * 2))
+#pragma unroll
+                for (int i = 0; i < DB; ++i) {
+                    const f4 x = odd_values<T>(v + (16 * i + 4 * g) * 2);
+#pragma unroll
+                    for (int b = 0; b < RB; ++b)
+                        if (k < seen[b]) o[b][i] += x;
+                }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const float sum = wave_sum16_groups(l[b]);
+        const int row = 16 * (wave * RB + b) + j;
+        if (row < it.rows)
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+                store<T, D, PREFIX>(p, it, row, 16 * i + 4 * g, o[b][i], m[b], sum);
     }
 }
 
@@ -603,28 +863,33 @@ static Range ranges(long long items, int keys, int step, int most) {
 }
 
 struct Plan {
-    bool single;
+    bool single;            // every sequence has at most sixteen rows
+    int rows, prefix_rows;  // rows of a work item
     int tiles, prefix_tiles;
     Range own, prefix;
-    int prefix_splits() const { return prefix.splits; }
     int slots() const { return own.splits + prefix.splits; }
 };
 
+static int tile_rows(int dim) { return dim > 128 ? TileShape<256>::kRows : TileShape<128>::kRows; }
+
 static Plan plan(const Attention& a) {
     Plan p;
-    const int kv = (int)a.pages.kv_heads, group = a.heads / kv;
-    const int step = (a.dtype == XATTN_F32 ? 16 : 32) * (a.pages.dim > 256 ? 1 : kWaves);
-    const long long rows = (long long)a.batch.tokens * group;
-    p.single = (long long)a.max_q * group <= kRows;
+    const int kv = (int)a.pages.kv_heads, group = a.heads / kv, dim = a.pages.dim;
+    const bool tiled = a.dtype != XATTN_F32 && dim <= 256;  // cache_tile_kernel takes it
+    const int few = (a.dtype == XATTN_F32 ? 16 : 32) * (dim > 256 ? 1 : kWaves);
+    const int many = dim > 128 ? TileShape<256>::kKeys : TileShape<128>::kKeys;
+    const long long rows = (long long)a.batch.tokens * group, most = (long long)a.max_q * group;
+    p.single = most <= kRows;
+    p.rows = tiled && most > kManyRows ? tile_rows(dim) : kRows;
     p.tiles = p.single ? a.batch.batch
-                       : (int)std::min<long long>(rows / kRows + a.batch.batch,
-                                                  ((long long)a.max_q * group + kRows - 1) /
-                                                      kRows * a.batch.batch);
-    p.own = ranges((long long)p.tiles * kv, a.max_kv, step, kMaxSlots / 2);
-    p.prefix_tiles = (int)((rows + kRows - 1) / kRows);
-    p.prefix = a.prefix_len > 0
-                   ? ranges((long long)p.prefix_tiles * kv, a.prefix_len, step, kMaxSlots / 2)
-                   : Range{0, 1};
+                       : (int)std::min<long long>(rows / p.rows + a.batch.batch,
+                                                  (most + p.rows - 1) / p.rows * a.batch.batch);
+    p.own = ranges((long long)p.tiles * kv, a.max_kv, p.rows > kRows ? many : few, kMaxSlots / 2);
+    p.prefix_rows = tiled && rows > kManyRows ? tile_rows(dim) : kRows;
+    p.prefix_tiles = (int)((rows + p.prefix_rows - 1) / p.prefix_rows);
+    p.prefix = a.prefix_len > 0 ? ranges((long long)p.prefix_tiles * kv, a.prefix_len,
+                                         p.prefix_rows > kRows ? many : few, kMaxSlots / 2)
+                                : Range{0, 1};
     return p;
 }
 
@@ -637,20 +902,29 @@ size_t attention_scratch(const Attention& a) {
     return parts(a, plan(a)) * (a.pages.dim * sizeof(float) + sizeof(float2));
 }
 
+template <typename T, int D, bool PREFIX>
+static void attend(const AttendParams& p, int rows, hipStream_t stream) {
+    const unsigned grid = p.pages.kv_heads * (unsigned)p.tiles * (unsigned)p.splits;
+    if constexpr (sizeof(T) == 2 && D <= 256)
+        if (rows > kRows) {
+            cache_tile_kernel<T, D, PREFIX><<<grid, 256, 0, stream>>>(p);
+            return;
+        }
+    cache_attend_kernel<T, D, PREFIX><<<grid, 256, 0, stream>>>(p);
+}
+
 template <typename T, int D>
 static void go(AttendParams& p, const Plan& plan, hipStream_t stream) {
-    const unsigned kv = p.pages.kv_heads;
     if (plan.prefix.splits > 0) {
         AttendParams f = p;
+        f.single = 0;
         f.tiles = plan.prefix_tiles;
         f.splits = plan.prefix.splits;
         f.chunk = plan.prefix.chunk;
         f.slot = 0;
-        cache_attend_kernel<T, D, true>
-            <<<kv * plan.prefix_tiles * plan.prefix.splits, 256, 0, stream>>>(f);
+        attend<T, D, true>(f, plan.prefix_rows, stream);
     }
-    cache_attend_kernel<T, D, false>
-        <<<kv * plan.tiles * plan.own.splits, 256, 0, stream>>>(p);
+    attend<T, D, false>(p, plan.rows, stream);
     if (p.po)
         cache_merge_kernel<T, D><<<(unsigned)p.batch.tokens * p.heads, 256, 0, stream>>>(
             p, plan.prefix.splits);
