@@ -28,6 +28,7 @@
 // nothing is read that no row sees; keys that some rows of a tile do not see get
 // the weight zero there.
 #include <algorithm>
+#include <cmath>
 
 #include "xattn_cache.h"
 #include "xattn_launch.h"
@@ -48,7 +49,9 @@ struct AttendParams {
     const void* q;
     void* out;
     long long qs, os;
-    float c2;         // scale * log2(e): scores in base-2 exponents
+    float c2;         // |scale| log2(e), not zero: scores to base-2 exponents
+    unsigned sign;    // flips the sign of q's elements where the scale is negative
+    float lag;        // kLag in scores
     int causal;
     int tiles;        // row tiles of a (kv head, range), at most
     int single;       // every sequence has one row tile: tile b is sequence b
@@ -84,8 +87,8 @@ __device__ inline f4 mfma4(float a, float b, f4 c) {
 
 template <typename T>
 __device__ inline unsigned pack2(float lo, float hi) {
-    const T a = (T)lo, b = (T)hi;
-    return (unsigned)__builtin_bit_cast(u16, a) | (unsigned)__builtin_bit_cast(u16, b) << 16;
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{lo, hi}, T2));
 }
 
 // Infinities and NaN in V.  A weight of zero does not silence them in a matrix
@@ -245,6 +248,14 @@ __device__ inline bool find_item(const AttendParams& p, Item* it) {
         it->table = p.batch.page_table + (long long)b * p.batch.width;
     }
     it->causal = !PREFIX && p.causal;
+    // The same in every lane, which the compiler cannot see.
+    it->s.first = __builtin_amdgcn_readfirstlane(it->s.first);
+    it->s.end = __builtin_amdgcn_readfirstlane(it->s.end);
+    it->s.last = __builtin_amdgcn_readfirstlane(it->s.last);
+    it->s.len = __builtin_amdgcn_readfirstlane(it->s.len);
+    it->s.bad = __builtin_amdgcn_readfirstlane(it->s.bad);
+    it->table = uniform_ptr(it->table);
+    local = __builtin_amdgcn_readfirstlane(local);
     const long long all = (long long)(it->s.end - it->s.first) * p.group.d;
     const long long row0 = (long long)local * ROWS;
     if (row0 >= all) return false;
@@ -316,7 +327,7 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
 
     // Lane j's row.  Rows behind the last repeat it and are not stored.
     const Row mine = it.row(p, min(j, rows - 1));
-    const int seen = s.seen(mine.token, it.causal);
+    const int seen = min(s.seen(mine.token, it.causal), k1);
 
     const int col0 = SHARED ? wave * DW : 0;
     u4 qr[NR];
@@ -324,7 +335,8 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
         const T* q = (const T*)p.q + mine.token * p.qs + (long long)mine.head * D + col0;
 #pragma unroll
         for (int r = 0; r < NR / (WIDE ? 1 : 2); ++r)
-            qr[r] = WIDE ? *(const u4*)(q + 16 * r + 4 * g) : *(const u4*)(q + 32 * r + 8 * g);
+            qr[r] = (WIDE ? *(const u4*)(q + 16 * r + 4 * g) : *(const u4*)(q + 32 * r + 8 * g)) ^
+                    p.sign;
     }
 
     f4 o[NB];
@@ -437,21 +449,22 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
             }
             // softmax
             const bool partial = k + KT > least;  // some row does not see all of the tile
+            if (partial)
+#pragma unroll
+                for (int h = 0; h < KT / 16; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (k + 16 * h + 4 * g + i >= seen) sc[h][i] = -INFINITY;
             float top = -INFINITY;
 #pragma unroll
             for (int h = 0; h < KT / 16; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = sc[h][i] * p.c2;
-                    if (partial && k + 16 * h + 4 * g + i >= min(seen, k1)) x = -INFINITY;
-                    sc[h][i] = x;
-                    top = fmaxf(top, x);
-                }
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[h][i]);
             top = fmaxf(m, wave_max16_groups(top));
             // exponents are taken from 0 while a row has seen nothing
-            const float ref = top == -INFINITY ? 0.0f : top;
+            const float ref = top == -INFINITY ? 0.0f : top * p.c2;
             if (__ballot(top != m)) {
-                const float keep = fast_exp2(m - ref);
+                const float keep = fast_exp2(m * p.c2 - ref);
                 l *= keep;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) o[b] *= keep;
@@ -461,7 +474,7 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
             for (int h = 0; h < KT / 16; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    sc[h][i] = fast_exp2(sc[h][i] - ref);
+                    sc[h][i] = fast_exp2(__builtin_fmaf(sc[h][i], p.c2, -ref));
                     l += sc[h][i];
                 }
             // product with V
@@ -519,7 +532,7 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
     if (__ballot(bad)) l = NAN;
 
     // Join the wavefronts' parts (of one maximum where they share their keys).
-    if (lane < 16) stats[wave][lane] = {m, l};
+    if (lane < 16) stats[wave][lane] = {m * p.c2, l};
     if constexpr (!SHARED) {
         float* part = (float*)vt + j * S::kORow;
 #pragma unroll
@@ -546,9 +559,9 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             store<T, D, PREFIX>(p, it, j, col0 + 16 * b + 16 * g + 4 * i,
-                                  f4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]}, m, l);
+                                  f4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]}, m * p.c2, l);
                 } else {
-                    store<T, D, PREFIX>(p, it, j, col0 + 16 * b + 4 * g, o[b], m, l);
+                    store<T, D, PREFIX>(p, it, j, col0 + 16 * b + 4 * g, o[b], m * p.c2, l);
                 }
             }
     } else {
@@ -614,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
         seen[b] = min(s.seen(r.token, it.causal), k1);
         const T* from = (const T*)p.q + r.token * p.qs + (long long)r.head * D + 8 * g;
 #pragma unroll
-        for (int i = 0; i < DS; ++i) q[b][i] = *(const u4*)(from + 32 * i);
+        for (int i = 0; i < DS; ++i) q[b][i] = *(const u4*)(from + 32 * i) ^ p.sign;
     }
     f4 o[RB][DB];
     float m[RB], l[RB];
@@ -705,31 +718,32 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
         u4 w[RB][KB / 2];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
+            if (partial)
+#pragma unroll
+                for (int h = 0; h < KB; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (k + 16 * h + 4 * g + i >= seen[b]) sc[b][h][i] = -INFINITY;
             float top = -INFINITY;
 #pragma unroll
             for (int h = 0; h < KB; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = sc[b][h][i] * p.c2;
-                    if (partial && k + 16 * h + 4 * g + i >= seen[b]) x = -INFINITY;
-                    sc[b][h][i] = x;
-                    top = fmaxf(top, x);
-                }
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[b][h][i]);
             top = wave_max16_groups(top);
-            if (__ballot(top > m[b] + kLag)) {
+            if (__ballot(top > m[b] + p.lag)) {
                 top = fmaxf(m[b], top);
-                const float keep = top == -INFINITY ? 1.0f : fast_exp2(m[b] - top);
+                const float keep = top == -INFINITY ? 1.0f : fast_exp2((m[b] - top) * p.c2);
                 l[b] *= keep;
 #pragma unroll
                 for (int i = 0; i < DB; ++i) o[b][i] *= keep;
                 m[b] = top;
             }
-            const float ref = m[b] == -INFINITY ? 0.0f : m[b];
+            const float ref = m[b] == -INFINITY ? 0.0f : m[b] * p.c2;
 #pragma unroll
             for (int h = 0; h < KB; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    sc[b][h][i] = fast_exp2(sc[b][h][i] - ref);
+                    sc[b][h][i] = fast_exp2(__builtin_fmaf(sc[b][h][i], p.c2, -ref));
                     l[b] += sc[b][h][i];
                 }
 #pragma unroll
@@ -780,7 +794,7 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
         if (row < it.rows)
 #pragma unroll
             for (int i = 0; i < DB; ++i)
-                store<T, D, PREFIX>(p, it, row, 16 * i + 4 * g, o[b][i], m[b], sum);
+                store<T, D, PREFIX>(p, it, row, 16 * i + 4 * g, o[b][i], m[b] * p.c2, sum);
     }
 }
 
@@ -951,7 +965,11 @@ bool launch_attention(const Attention& a, void* scratch, hipStream_t stream) {
     p.out = a.out;
     p.qs = a.qs;
     p.os = a.os;
-    p.c2 = a.scale * kLog2e;
+    // A scale of zero makes all scores equal; so does one that is next to it, and a
+    // masked score's -infinity stays one.
+    p.c2 = std::max(std::fabs(a.scale) * kLog2e, 1e-37f);
+    p.lag = std::min(kLag / p.c2, 1e30f);
+    p.sign = a.scale >= 0 ? 0 : a.dtype == XATTN_F32 ? 0x80000000u : 0x80008000u;
     p.causal = a.causal;
     p.tiles = pl.tiles;
     p.single = pl.single;
