@@ -1,6 +1,7 @@
 // C entry points of kernels.so: argument validation, error state, device
 // queries, workspace and launch planning.  The kernels live in the other
-// translation units; every launcher here is host code only.
+// translation units (those of the cache operators come in at the end of this
+// one, xattn_cache_abi.h); every launcher here is host code only.
 #include <stdarg.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -962,3 +963,6 @@ void launch_wmma_splitk_bf16_kernel(const uint16_t* Q, const uint16_t* K, const 
 }
 
 }  // extern "C"
+
+// The operators of a key/value cache: their entry points and kernels.
+#include "xattn_cache_abi.h"

@@ -1,4 +1,4 @@
-// Shared pieces of the cache operators (xattn_rope.hip, xattn_cache.hip): the
+// Shared pieces of the cache operators (xattn_rope.h, xattn_cache_attend.h): the
 // kernels' views of a paged cache and of a ragged batch, and the look-ups in
 // them.  Every look-up is bounded by the host's sizes whatever the device
 // arrays hold.
@@ -52,7 +52,7 @@ struct Rope {
 
 constexpr int kMaxRot = 2048;  // rotated elements of a head: their angles fit LDS
 
-// Launchers; the arguments are valid (xattn_cache_abi.hip).
+// Launchers; the arguments are valid (xattn_cache_abi.h).
 bool launch_rope(const void* x, void* y, const int* positions, const Rope& rope, int dtype,
                  int tokens, int heads, int dim, long long xs, long long ys,
                  hipStream_t stream);

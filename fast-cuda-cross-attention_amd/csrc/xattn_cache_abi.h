@@ -1,11 +1,13 @@
 // C entry points of the cache operators: argument checks and the views the
-// kernels take (xattn_rope.hip, xattn_cache.hip).  Host code only.
+// kernels take (xattn_rope.h, xattn_cache_attend.h).  Host code only.
+#pragma once
+
 #include <math.h>
 
 #include <algorithm>
 
-#include "xattn_cache.h"
-#include "xattn_launch.h"
+#include "xattn_cache_attend.h"
+#include "xattn_rope.h"
 
 namespace xattn {
 namespace cache {
@@ -191,12 +193,6 @@ static void attention(const char* who, const xattn_kv_cache* cache, const xattn_
     launch_attention(a, scratch, stream);
 }
 
-}  // namespace cache
-}  // namespace xattn
-
-using namespace xattn;
-using namespace xattn::cache;
-
 extern "C" {
 
 int xattn_rope_frequencies(double* freqs, int rot_dim, double base, int scaling, double factor,
@@ -336,3 +332,6 @@ void launch_prefix_attention_kernel(const xattn_kv_cache* cache, const xattn_bat
 }
 
 }  // extern "C"
+
+}  // namespace cache
+}  // namespace xattn

@@ -27,6 +27,8 @@
 // Keys beyond the last row's reach are read from the last key within it, so that
 // nothing is read that no row sees; keys that some rows of a tile do not see get
 // the weight zero there.
+#pragma once
+
 #include <algorithm>
 #include <cmath>
 
@@ -80,6 +82,12 @@ __device__ inline f4 mfma32(u4 a, u4 b, f4 c) {
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a),
                                                        __builtin_bit_cast(V, b), c, 0, 0, 0);
+}
+// Eight ones: their product with the weights sums them, over all lanes of a row.
+template <typename T>
+__device__ inline u4 ones() {
+    const unsigned two = __is_same(T, __bf16) ? 0x3f803f80u : 0x3c003c00u;
+    return u4{two, two, two, two};
 }
 __device__ inline f4 mfma4(float a, float b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -602,15 +610,17 @@ struct TileShape {
     static constexpr int kKeys = D > 128 ? 32 : 64;       // keys of a tile
     static constexpr int kPieces = D / 8;                 // 16-byte pieces of a row
     static constexpr int kLoads = kKeys * kPieces / 256;  // pieces of a thread, of K and of V
-    static constexpr int kLdsRow = D * 2 + 32;
-    static constexpr int kTile = kKeys * kLdsRow;
+    static constexpr int kTile = kKeys * D * 2;           // bytes of a tile in LDS
+    // What a row's piece numbers are xored with in LDS: rows 0 .. 7 put a column's
+    // 32 bytes into eight different eighths of the banks.
+    static __device__ int swizzle(int row) { return D == 64 ? row / 2 % 4 * 2 : row % 8 * 2; }
 };
 
 template <typename T, int D, bool PREFIX>
 __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
     typedef TileShape<D> S;
     constexpr int RB = S::kBlocks, KT = S::kKeys, KB = KT / 16, NL = S::kLoads;
-    constexpr int DS = D / 32, DB = D / 16, LR = S::kLdsRow;
+    constexpr int DS = D / 32, DB = D / 16, LR = D * 2;
     __shared__ __align__(16) char lds[4 * S::kTile];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int j = lane % 16, g = lane / 16;
@@ -629,154 +639,194 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
 #pragma unroll
         for (int i = 0; i < DS; ++i) q[b][i] = *(const u4*)(from + 32 * i) ^ p.sign;
     }
-    f4 o[RB][DB];
-    float m[RB], l[RB];
+    f4 o[RB][DB], l[RB];  // l: the sum of a row's weights, four times
+    float m[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
         m[b] = -INFINITY;
-        l[b] = 0.0f;
+        l[b] = f4{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[b][i] = f4{0, 0, 0, 0};
     }
 
-    // A thread's pieces of a tile: piece threadIdx % kPieces of every so many-th row.
-    constexpr int STRIDE = 256 / S::kPieces;
-    const int piece = threadIdx.x % S::kPieces, first = threadIdx.x / S::kPieces;
+    // A wavefront's pieces of a tile: AT_ONCE rows to a DMA of 1 KiB, the workgroup
+    // STRIDE.  A row's pieces are permuted in LDS by swizzle(row): with rows whose
+    // bytes are a power of two, eight rows of one column would share their banks,
+    // and DMA leaves no room for padding.  Where AT_ONCE divides the page size its
+    // rows lie on one page, and their address is one scalar plus a lane's constant
+    // offset; a lane's own address otherwise, and where rows behind the last key
+    // repeat it.
+    constexpr int AT_ONCE = 64 / S::kPieces, STRIDE = kWaves * AT_ONCE;
+    const int wave_row = __builtin_amdgcn_readfirstlane(wave * AT_ONCE);
+    const int lane_row = lane / S::kPieces;
+    const unsigned lane_byte =
+        16u * (lane % S::kPieces ^ S::swizzle(wave * AT_ONCE + lane_row));
+    const bool runs = p.pages.page_size.d % AT_ONCE == 0;
+    const unsigned size = p.pages.page_size.d;
     bool bad = false, odd = false;
-    int id[NL];
-    unsigned slot[NL];
+    int id[NL];  // page of each piece of the next tile
     const auto find = [&](int k) {
+        const bool whole = runs && k + KT <= k1;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const unsigned key = (unsigned)min(k + first + STRIDE * i, k1 - 1);
-            const unsigned page = p.pages.page_size.div(key);
-            id[i] = it.table[page];
-            slot[i] = key - page * p.pages.page_size.d;
+            const int key = k + STRIDE * i + wave_row + (whole ? 0 : lane_row);
+            id[i] = it.table[p.pages.page_size.div((unsigned)min(key, k1 - 1))];
         }
     };
-    u4 kr[NL], vr[NL];
-    size_t at[NL];
-    const auto load_k = [&]() {
+    DmaSrc k_pool, v_pool;
+    dma_base2(p.pages.k, p.pages.v, k_pool, v_pool);
+    const unsigned lds0 = lds_u32(lds);
+    const auto load = [&](int t, int k) {
+        const unsigned to = lds0 + (t & 1) * 2 * S::kTile + wave_row * (D * 2);
+        if (runs && k + KT <= k1) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const bool ok = id[i] >= 0 && (unsigned)id[i] < p.pages.num_pages;
-            bad |= !ok;
-            at[i] = (size_t)(((ok ? (unsigned)id[i] : 0u) * p.pages.kv_heads + it.kv_head) *
-                                 p.pages.page_size.d + slot[i]) * (D * 2) + 16 * piece;
-            kr[i] = *(const u4*)(p.pages.k + at[i]);
+            for (int i = 0; i < NL; ++i) {
+                const unsigned key = (unsigned)(k + STRIDE * i + wave_row);
+                const int page = __builtin_amdgcn_readfirstlane(id[i]);
+                const bool ok = page >= 0 && (unsigned)page < p.pages.num_pages;
+                bad |= !ok;
+                const unsigned row = ((ok ? (unsigned)page : 0u) * p.pages.kv_heads + it.kv_head) *
+                                         size + (key - p.pages.page_size.div(key) * size);
+                const size_t at = (size_t)row * (D * 2);
+                const unsigned from = lane_row * (D * 2) + lane_byte;
+                dma16_m0<0>(k_pool + at, from, to + i * STRIDE * (D * 2));
+                dma16_m0<0>(v_pool + at, from, to + S::kTile + i * STRIDE * (D * 2));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const unsigned key = (unsigned)min(k + STRIDE * i + wave_row + lane_row, k1 - 1);
+                const bool ok = id[i] >= 0 && (unsigned)id[i] < p.pages.num_pages;
+                bad |= !ok;
+                const unsigned row = ((ok ? (unsigned)id[i] : 0u) * p.pages.kv_heads + it.kv_head) *
+                                         size + (key - p.pages.page_size.div(key) * size);
+                const size_t at = (size_t)row * (D * 2) + lane_byte;
+                dma16_lanes(p.pages.k + at, to + i * STRIDE * (D * 2));
+                dma16_lanes(p.pages.v + at, to + S::kTile + i * STRIDE * (D * 2));
+            }
         }
     };
-    const auto load_v = [&]() {
+    // The tile loaded last has arrived for this wavefront; infinities and NaN in
+    // its pieces of V are cleared if some rows do not see all of the tile.
+    const auto arrived = [&](int t, int k) {
+        wait_vmcnt<0>();
+        if (k + KT > it.least)
 #pragma unroll
-        for (int i = 0; i < NL; ++i) vr[i] = *(const u4*)(p.pages.v + at[i]);
-    };
-    char* const mine = lds + first * LR + 16 * piece;
-    const auto put_k = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < NL; ++i)
-            *(u4*)(mine + (t & 1) * 2 * S::kTile + i * STRIDE * LR) = kr[i];
-    };
-    const auto put_v = [&](int t, bool partial) {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            if (partial) odd |= clear_not_finite<T>(vr[i]);
-            *(u4*)(mine + ((t & 1) * 2 + 1) * S::kTile + i * STRIDE * LR) = vr[i];
-        }
+            for (int i = 0; i < NL; ++i) {
+                u4* at = (u4*)(lds + ((t & 1) * 2 + 1) * S::kTile +
+                               (wave_row + i * STRIDE) * (D * 2) + lane * 16);
+                u4 x = *at;
+                if (clear_not_finite<T>(x)) {
+                    odd = true;
+                    *at = x;
+                }
+            }
     };
 
     if (k0 < k1) {
         find(k0);
-        load_k();
-        load_v();
+        load(0, k0);
         find(k0 + KT);
-        put_k(0);
-        put_v(0, k0 + KT > it.least);
+        arrived(0, k0);
     }
-    __syncthreads();
+    lds_barrier();
     int t = 0;
     for (int k = k0; k < k1; k += KT, ++t) {
         const bool more = k + KT < k1;
         if (more) {
-            load_k();
+            load(t + 1, k + KT);
             find(k + 2 * KT);
         }
         const char* kt = lds + (t & 1) * 2 * S::kTile;
         const char* vt = kt + S::kTile;
         f4 sc[RB][KB];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int h = 0; h < KB; ++h) {
 #pragma unroll
             for (int b = 0; b < RB; ++b) sc[b][h] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < DS; ++i) {
-                const u4 a = *(const u4*)(kt + (16 * h + j) * LR + 64 * i + 16 * g);
+                const u4 a = *(const u4*)(kt + (16 * h + j) * LR + 16 * (4 * i + g ^ S::swizzle(j)));
 #pragma unroll
                 for (int b = 0; b < RB; ++b) sc[b][h] = mfma32<T>(a, q[b][i], sc[b][h]);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         const bool partial = k + KT > it.least;
-        u4 w[RB][KB / 2];
+        if (partial) {
+            int key = k + 4 * g;
+            asm volatile("" : "+v"(key));  // keeps the comparisons in this branch
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            if (partial)
+            for (int b = 0; b < RB; ++b)
 #pragma unroll
                 for (int h = 0; h < KB; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (k + 16 * h + 4 * g + i >= seen[b]) sc[b][h][i] = -INFINITY;
-            float top = -INFINITY;
+                        if (key + 16 * h + i >= seen[b]) sc[b][h][i] = -INFINITY;
+        }
+        float top[RB];
+        bool past = false;
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            top[b] = -INFINITY;
 #pragma unroll
             for (int h = 0; h < KB; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[b][h][i]);
-            top = wave_max16_groups(top);
-            if (__ballot(top > m[b] + p.lag)) {
-                top = fmaxf(m[b], top);
-                const float keep = top == -INFINITY ? 1.0f : fast_exp2((m[b] - top) * p.c2);
+                for (int i = 0; i < 4; ++i) top[b] = fmaxf(top[b], sc[b][h][i]);
+            top[b] = wave_max16_groups(top[b]);
+            past |= top[b] > m[b] + p.lag;
+        }
+        if (__ballot(past))
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                const float to = fmaxf(m[b], top[b]);
+                const float keep = to == -INFINITY ? 1.0f : fast_exp2((m[b] - to) * p.c2);
                 l[b] *= keep;
 #pragma unroll
                 for (int i = 0; i < DB; ++i) o[b][i] *= keep;
-                m[b] = top;
+                m[b] = to;
             }
+        u4 w[RB][KB / 2];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
             const float ref = m[b] == -INFINITY ? 0.0f : m[b] * p.c2;
 #pragma unroll
             for (int h = 0; h < KB; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 4; ++i)
                     sc[b][h][i] = fast_exp2(__builtin_fmaf(sc[b][h][i], p.c2, -ref));
-                    l[b] += sc[b][h][i];
-                }
 #pragma unroll
-            for (int h = 0; h < KB / 2; ++h)
+            for (int h = 0; h < KB / 2; ++h) {
                 w[b][h] = u4{pack2<T>(sc[b][2 * h][0], sc[b][2 * h][1]),
                              pack2<T>(sc[b][2 * h][2], sc[b][2 * h][3]),
                              pack2<T>(sc[b][2 * h + 1][0], sc[b][2 * h + 1][1]),
                              pack2<T>(sc[b][2 * h + 1][2], sc[b][2 * h + 1][3])};
+                l[b] = mfma32<T>(ones<T>(), w[b][h], l[b]);
+            }
         }
-        if (more) {
-            put_k(t + 1);
-            load_v();
-        }
-        lds_s4* from = (lds_s4*)(vt + (4 * g + j / 4) * LR + j % 4 * 8);
+        const int row = 4 * g + j / 4;  // of this lane's pieces of V
 #pragma unroll
-        for (int h = 0; h < KB / 2; ++h)
+        for (int i = 0; i < DB; ++i) {
+            lds_s4* from = (lds_s4*)(vt + row * LR + 16 * (2 * i + j % 4 / 2 ^ S::swizzle(row)) +
+                                     j % 2 * 8);
 #pragma unroll
-            for (int i = 0; i < DB; ++i) {
-                const s4 lo =
-                    __builtin_amdgcn_ds_read_tr16_b64_v4i16(from + 4 * i + 32 * h * LR / 8);
+            for (int h = 0; h < KB / 2; ++h) {
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(from + 32 * h * LR / 8);
                 const s4 hi =
-                    __builtin_amdgcn_ds_read_tr16_b64_v4i16(from + 4 * i + (32 * h + 16) * LR / 8);
+                    __builtin_amdgcn_ds_read_tr16_b64_v4i16(from + (32 * h + 16) * LR / 8);
                 const u4 a = __builtin_bit_cast(
                     u4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
                 for (int b = 0; b < RB; ++b) o[b][i] = mfma32<T>(a, w[b][h], o[b][i]);
             }
-        if (more) put_v(t + 1, k + 2 * KT > it.least);
+        }
+        if (more) arrived(t + 1, k + KT);
         lds_barrier();
     }
     if (__syncthreads_or(bad))
 #pragma unroll
-        for (int b = 0; b < RB; ++b) l[b] = NAN;
+        for (int b = 0; b < RB; ++b) l[b][0] = NAN;
     if (__syncthreads_or(odd))
         for (int k = max(k0, it.least / KT * KT); k < k1; ++k)
             if (const char* v = it.row_of_v(p, k, D * 2))
@@ -789,12 +839,11 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
                 }
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-        const float sum = wave_sum16_groups(l[b]);
         const int row = 16 * (wave * RB + b) + j;
         if (row < it.rows)
 #pragma unroll
             for (int i = 0; i < DB; ++i)
-                store<T, D, PREFIX>(p, it, row, 16 * i + 4 * g, o[b][i], m[b] * p.c2, sum);
+                store<T, D, PREFIX>(p, it, row, 16 * i + 4 * g, o[b][i], m[b] * p.c2, l[b][0]);
     }
 }
 

@@ -192,6 +192,16 @@ __device__ inline void dma16_m0(DmaSrc src, unsigned voff, unsigned lds_byte) {
         : "memory");
 }
 
+// The same with an address of its own for every lane.
+__device__ inline void dma16_lanes(const void* src, unsigned lds_byte) {
+    asm volatile(
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, off"
+        :
+        : "v"(src), "{m0}"(lds_byte)
+        : "memory");
+}
+
 // --------------------------------------------------------------------------
 // Phase clock: instrumented builds only (`make phaseclock` defines
 // XATTN_PHASE_CLOCK; the product build compiles none of it).  A kernel

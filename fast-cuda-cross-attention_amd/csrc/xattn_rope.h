@@ -12,6 +12,8 @@
 // sines in LDS, each once for all of the token's heads, and then moves the
 // heads in 16-byte pieces, both halves of a pair in one thread, so that y may
 // be x.
+#pragma once
+
 #include <algorithm>
 
 #include "xattn_cache.h"
