@@ -664,46 +664,46 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
     const bool runs = p.pages.page_size.d % AT_ONCE == 0;
     const unsigned size = p.pages.page_size.d;
     bool bad = false, odd = false;
-    int id[NL];  // page of each piece of the next tile
+    int ids;  // lane's page of the next tile: that of its key lane % KT
     const auto find = [&](int k) {
-        const bool whole = runs && k + KT <= k1;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int key = k + STRIDE * i + wave_row + (whole ? 0 : lane_row);
-            id[i] = it.table[p.pages.page_size.div((unsigned)min(key, k1 - 1))];
-        }
+        ids = it.table[p.pages.page_size.div((unsigned)min(k + lane % KT, k1 - 1))];
     };
     DmaSrc k_pool, v_pool;
     dma_base2(p.pages.k, p.pages.v, k_pool, v_pool);
     const unsigned lds0 = lds_u32(lds);
-    const auto load = [&](int t, int k) {
-        const unsigned to = lds0 + (t & 1) * 2 * S::kTile + wave_row * (D * 2);
-        if (runs && k + KT <= k1) {
+    // A tile's i-th pieces of K and V.  Whole tiles of pages as above: their
+    // sources and the destination are prepared together, then asked for.
+    struct Piece1 {
+        DmaSrc k, v;
+        unsigned to;
+    };
+    const unsigned from = lane_row * (D * 2) + lane_byte;
+    const auto piece = [&](int t, int k, int i) {
+        const int at_row = STRIDE * i + wave_row;
+        const unsigned key = (unsigned)(k + at_row);
+        const int page = __builtin_amdgcn_readlane(ids, at_row);
+        const bool ok = page >= 0 && (unsigned)page < p.pages.num_pages;
+        bad |= !ok;
+        const unsigned row = ((ok ? (unsigned)page : 0u) * p.pages.kv_heads + it.kv_head) * size +
+                             (key - p.pages.page_size.div(key) * size);
+        const size_t at = (size_t)row * (D * 2);
+        return Piece1{k_pool + at, v_pool + at,
+                      lds0 + (t & 1) * 2 * S::kTile + at_row * (D * 2)};
+    };
+    const auto load_any = [&](int t, int k) {
 #pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const unsigned key = (unsigned)(k + STRIDE * i + wave_row);
-                const int page = __builtin_amdgcn_readfirstlane(id[i]);
-                const bool ok = page >= 0 && (unsigned)page < p.pages.num_pages;
-                bad |= !ok;
-                const unsigned row = ((ok ? (unsigned)page : 0u) * p.pages.kv_heads + it.kv_head) *
-                                         size + (key - p.pages.page_size.div(key) * size);
-                const size_t at = (size_t)row * (D * 2);
-                const unsigned from = lane_row * (D * 2) + lane_byte;
-                dma16_m0<0>(k_pool + at, from, to + i * STRIDE * (D * 2));
-                dma16_m0<0>(v_pool + at, from, to + S::kTile + i * STRIDE * (D * 2));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const unsigned key = (unsigned)min(k + STRIDE * i + wave_row + lane_row, k1 - 1);
-                const bool ok = id[i] >= 0 && (unsigned)id[i] < p.pages.num_pages;
-                bad |= !ok;
-                const unsigned row = ((ok ? (unsigned)id[i] : 0u) * p.pages.kv_heads + it.kv_head) *
-                                         size + (key - p.pages.page_size.div(key) * size);
-                const size_t at = (size_t)row * (D * 2) + lane_byte;
-                dma16_lanes(p.pages.k + at, to + i * STRIDE * (D * 2));
-                dma16_lanes(p.pages.v + at, to + S::kTile + i * STRIDE * (D * 2));
-            }
+        for (int i = 0; i < NL; ++i) {
+            const int at_row = STRIDE * i + wave_row;
+            const unsigned to = lds0 + (t & 1) * 2 * S::kTile + at_row * (D * 2);
+            const unsigned key = (unsigned)min(k + at_row + lane_row, k1 - 1);
+            const int page = __shfl(ids, at_row + lane_row);
+            const bool ok = page >= 0 && (unsigned)page < p.pages.num_pages;
+            bad |= !ok;
+            const unsigned row = ((ok ? (unsigned)page : 0u) * p.pages.kv_heads + it.kv_head) *
+                                     size + (key - p.pages.page_size.div(key) * size);
+            const size_t at = (size_t)row * (D * 2) + lane_byte;
+            dma16_lanes(p.pages.k + at, to);
+            dma16_lanes(p.pages.v + at, to + S::kTile);
         }
     };
     // The tile loaded last has arrived for this wavefront; infinities and NaN in
@@ -725,7 +725,7 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
 
     if (k0 < k1) {
         find(k0);
-        load(0, k0);
+        load_any(0, k0);
         find(k0 + KT);
         arrived(0, k0);
     }
@@ -733,25 +733,49 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
     int t = 0;
     for (int k = k0; k < k1; k += KT, ++t) {
         const bool more = k + KT < k1;
-        if (more) {
-            load(t + 1, k + KT);
-            find(k + 2 * KT);
-        }
         const char* kt = lds + (t & 1) * 2 * S::kTile;
         const char* vt = kt + S::kTile;
         f4 sc[RB][KB];
+        u4 a[2][DS];
+        const auto read_k = [&](int h) {
+#pragma unroll
+            for (int i = 0; i < DS; ++i)
+                a[h & 1][i] =
+                    *(const u4*)(kt + (16 * h + j) * LR + 16 * (4 * i + g ^ S::swizzle(j)));
+        };
+        const auto scores = [&](int h, int from, int to) {
+#pragma unroll
+            for (int i = from; i < to; ++i)
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+                    sc[b][h] = mfma32<T>(a[h & 1][i], q[b][i], i ? sc[b][h] : f4{0, 0, 0, 0});
+        };
         __builtin_amdgcn_s_setprio(1);
+        read_k(0);
+        if (runs && k + 2 * KT <= k1) {
+            // The next tile is asked for piece by piece between the products (the
+            // path to memory takes a wavefront's requests no faster), each read of
+            // LDS before the requests that it need not wait for.
 #pragma unroll
-        for (int h = 0; h < KB; ++h) {
+            for (int h = 0; h < KB; ++h) {
+                if (h + 1 < KB) read_k(h + 1);
 #pragma unroll
-            for (int b = 0; b < RB; ++b) sc[b][h] = f4{0, 0, 0, 0};
+                for (int i = h * NL / KB; i < (h + 1) * NL / KB; ++i) {
+                    const Piece1 x = piece(t + 1, k + KT, i);
+                    dma16_m0<0>(x.k, from, x.to);
+                    dma16_m0<0>(x.v, from, x.to + S::kTile);
+                }
+                scores(h, 0, DS);
+            }
+        } else {
+            if (more) load_any(t + 1, k + KT);
 #pragma unroll
-            for (int i = 0; i < DS; ++i) {
-                const u4 a = *(const u4*)(kt + (16 * h + j) * LR + 16 * (4 * i + g ^ S::swizzle(j)));
-#pragma unroll
-                for (int b = 0; b < RB; ++b) sc[b][h] = mfma32<T>(a, q[b][i], sc[b][h]);
+            for (int h = 0; h < KB; ++h) {
+                if (h + 1 < KB) read_k(h + 1);
+                scores(h, 0, DS);
             }
         }
+        if (more) find(k + 2 * KT);
         __builtin_amdgcn_s_setprio(0);
         const bool partial = k + KT > it.least;
         if (partial) {
