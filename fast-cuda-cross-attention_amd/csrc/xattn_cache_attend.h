@@ -222,18 +222,18 @@ struct Item {
 // ranges slowest, and of a ragged batch the ranges that few sequences have come
 // last.
 template <int ROWS, bool PREFIX>
-__device__ inline bool find_item(const AttendParams& p, Item* it) {
+__device__ inline bool find_item(const AttendParams& p, unsigned block, Item* it) {
     unsigned tile, stream;
     const unsigned streams = p.pages.kv_heads * p.splits;
     if (!p.single && streams % kNumXcd == 0) {
-        const unsigned at = blockIdx.x / kNumXcd;
-        stream = blockIdx.x % kNumXcd + at / p.tiles * kNumXcd;
+        const unsigned at = block / kNumXcd;
+        stream = block % kNumXcd + at / p.tiles * kNumXcd;
         tile = at % p.tiles;
         it->kv_head = stream % p.pages.kv_heads;
         it->split = (int)(stream / p.pages.kv_heads);
     } else {
-        const unsigned rest = blockIdx.x / p.pages.kv_heads;
-        it->kv_head = blockIdx.x % p.pages.kv_heads;
+        const unsigned rest = block / p.pages.kv_heads;
+        it->kv_head = block % p.pages.kv_heads;
         tile = rest % p.tiles;
         it->split = (int)(rest / p.tiles);
     }
@@ -314,21 +314,21 @@ struct Shape {
     static constexpr int kWaveLds =
         kCols > 1 ? kVTile : (kVTile > kRows * kORow * 4 ? kVTile : kRows * kORow * 4);
     static constexpr int kShare = kKeys * kRows * 4;    // bytes of a wavefront's share of scores
-    static constexpr int kLds = kWaves * kWaveLds + (kCols > 1 ? 2 * kWaves * kShare : 0);
+    static constexpr int kStats = kWaves * kRows * 8;   // their maxima and sums
+    static constexpr int kLds = kWaves * kWaveLds + (kCols > 1 ? 2 * kWaves * kShare : 0) + kStats;
 };
 
 template <typename T, int D, bool PREFIX>
-__global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
+__device__ __forceinline__ void attend_item(const AttendParams& p, unsigned block, char* lds) {
     typedef Shape<T, D> S;
     constexpr int KT = S::kKeys, DW = S::kDW, NR = S::kRegs, NB = S::kBlocks;
     constexpr bool WIDE = S::kWide, SHARED = S::kCols > 1;
-    __shared__ __align__(16) char lds[S::kLds];
-    __shared__ float2 stats[kWaves][kRows];
+    float2(*const stats)[kRows] = (float2(*)[kRows])(lds + S::kLds - S::kStats);
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int j = lane % 16, g = lane / 16;
 
     Item it;
-    if (!find_item<kRows, PREFIX>(p, &it)) return;
+    if (!find_item<kRows, PREFIX>(p, block, &it)) return;
     const Sequence& s = it.s;
     const int rows = it.rows, least = it.least, k0 = it.k0, k1 = it.k1;
     const unsigned kv_head = it.kv_head;
@@ -601,6 +601,13 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
 // when a score exceeds it by kLag (in exponents of 2), so that the output is
 // rarely rescaled; they stay below 2^kLag, far from the range of either type.
 // --------------------------------------------------------------------------
+#ifndef WANT_TILE
+#define WANT_TILE 4
+#define WANT_FEW 2
+#define WANT_SINGLE 4
+#define WANT_PREFIX 2
+#define TILE_STEP 4
+#endif
 constexpr float kLag = 8.0f;
 
 template <int D>
@@ -611,21 +618,21 @@ struct TileShape {
     static constexpr int kPieces = D / 8;                 // 16-byte pieces of a row
     static constexpr int kLoads = kKeys * kPieces / 256;  // pieces of a thread, of K and of V
     static constexpr int kTile = kKeys * D * 2;           // bytes of a tile in LDS
+    static constexpr int kLds = 4 * kTile;
     // What a row's piece numbers are xored with in LDS: rows 0 .. 7 put a column's
     // 32 bytes into eight different eighths of the banks.
     static __device__ int swizzle(int row) { return D == 64 ? row / 2 % 4 * 2 : row % 8 * 2; }
 };
 
 template <typename T, int D, bool PREFIX>
-__global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
+__device__ __forceinline__ void tile_item(const AttendParams& p, unsigned block, char* lds) {
     typedef TileShape<D> S;
     constexpr int RB = S::kBlocks, KT = S::kKeys, KB = KT / 16, NL = S::kLoads;
     constexpr int DS = D / 32, DB = D / 16, LR = D * 2;
-    __shared__ __align__(16) char lds[4 * S::kTile];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int j = lane % 16, g = lane / 16;
     Item it;
-    if (!find_item<S::kRows, PREFIX>(p, &it)) return;
+    if (!find_item<S::kRows, PREFIX>(p, block, &it)) return;
     const Sequence& s = it.s;
     const int k0 = it.k0, k1 = it.k1;
 
@@ -872,61 +879,111 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
 }
 
 // --------------------------------------------------------------------------
-// cache_merge_kernel: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the
-// parts of a row, in their order.  A workgroup takes a row; D / 4 threads hold
-// its columns, as many groups of them as fit take every so many-th part.
+// Kernels.  The keys of a prefix and those of the sequences are worked on in
+// one launch, the prefix's (longer) items first: the sequences' fill in.
 // --------------------------------------------------------------------------
-constexpr int kMaxSlots = 512;
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
+    __shared__ __align__(16) char lds[Shape<T, D>::kLds];
+    attend_item<T, D, false>(p, blockIdx.x, lds);
+}
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void cache_merge_kernel(AttendParams p, int prefix_splits) {
-    constexpr int TC = D / 4, GROUPS = 256 / TC;
-    __shared__ float weight[kMaxSlots];
-    __shared__ f4 sums[GROUPS > 1 ? 256 : 1];
-    __shared__ float total[2];
-    const int t = (int)(blockIdx.x / p.heads), head = (int)(blockIdx.x % p.heads);
+__global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
+    __shared__ __align__(16) char lds[TileShape<D>::kLds];
+    tile_item<T, D, false>(p, blockIdx.x, lds);
+}
+
+// TILES: how many of the two go by tile_item (2: both, 1: the prefix, 0: none).
+template <typename T, int D, int TILES>
+__global__ __launch_bounds__(256, TILES == 2 || (TILES == 1 && D <= 128) ? 2 : 1) void
+cache_prefix_kernel(
+    AttendParams prefix, AttendParams own, unsigned prefix_blocks) {
+    constexpr int few = TILES < 2 ? Shape<T, D>::kLds : 0;
+    constexpr int many = TILES > 0 ? TileShape<D>::kLds : 0;
+    __shared__ __align__(16) char lds[few > many ? few : many];
+    if (blockIdx.x < prefix_blocks) {
+        if constexpr (TILES > 0)
+            tile_item<T, D, true>(prefix, blockIdx.x, lds);
+        else
+            attend_item<T, D, true>(prefix, blockIdx.x, lds);
+    } else {
+        if constexpr (TILES > 1)
+            tile_item<T, D, false>(own, blockIdx.x - prefix_blocks, lds);
+        else
+            attend_item<T, D, false>(own, blockIdx.x - prefix_blocks, lds);
+    }
+}
+
+// --------------------------------------------------------------------------
+// cache_merge_kernel: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the
+// parts of a row.  A wavefront takes 256 columns of a row, or all of them, in
+// 64 / LANES groups of LANES lanes that take every so many-th part; with
+// `together` the four wavefronts of a workgroup share a row's parts (few rows of
+// many parts), otherwise each has a row of its own.
+// --------------------------------------------------------------------------
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cache_merge_kernel(AttendParams p, int prefix_parts,
+                                                          int together) {
+    constexpr int COLS = D > 256 ? 256 : D, LANES = COLS / 4, GROUPS = kWave / LANES;
+    __shared__ f4 sums[kWaves - 1][LANES];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const unsigned unit = together ? blockIdx.x : blockIdx.x * kWaves + wave;
+    const unsigned row = unit / (D / COLS), col = unit % (D / COLS) * COLS + lane % LANES * 4;
+    const int t = (int)(row / p.heads), head = (int)(row % p.heads);
+    if (t >= p.batch.tokens) return;
     const int b = token_sequence(p.batch, t);
     if (b >= p.batch.batch) return;
     const Sequence s = sequence(p.batch, b);
     if (t < s.first || t >= s.end) return;
     const int n = s.seen(t, p.causal);
     if (p.slot == 0 && (p.splits == 1 || n <= p.chunk)) return;  // stored already
-    int own = (n + p.chunk - 1) / p.chunk;
-    if (own > p.splits) own = p.splits;
-    const int parts = prefix_splits + own;
-    const size_t at = ((size_t)t * p.heads + head) * p.slots;
-    if (threadIdx.x < kWave) {
-        float top = -INFINITY, sum = 0.0f;
-        for (int i = threadIdx.x; i < parts; i += kWave) top = fmaxf(top, p.ml[at + i].x);
-        top = wave_max(top);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        for (int i = threadIdx.x; i < parts; i += kWave) {
-            const float2 ml = p.ml[at + i];
-            weight[i] = fast_exp2(ml.x - ref);
-            sum += weight[i] * ml.y;
-        }
-        sum = wave_sum(sum);
-        if (threadIdx.x == 0) total[0] = s.bad ? NAN : sum;
-    }
-    __syncthreads();
-    const int c = threadIdx.x % TC, grp = threadIdx.x / TC;
+    const int own = min((n + p.chunk - 1) / p.chunk, p.splits);
+    const int parts = prefix_parts + own;
+    const size_t at = (size_t)row * p.slots;
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += kWave) top = fmaxf(top, p.ml[at + i].x);
+    top = wave_max(top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
     f4 x = {0, 0, 0, 0};
-    if (grp < GROUPS)
+    const int first = lane / LANES + (together ? wave * GROUPS : 0);
+    const int step = GROUPS * (together ? kWaves : 1);
+    for (int from = 0; from < parts; from += kWave) {
+        float weight = 0.0f;
+        if (from + lane < parts) {
+            const float2 ml = p.ml[at + from + lane];
+            weight = fast_exp2(ml.x - ref);
+            sum += weight * ml.y;
+        }
+        const int count = min(kWave, parts - from);
 #pragma unroll 4
-        for (int i = grp; i < parts; i += GROUPS)
-            x += weight[i] * *(const f4*)(p.po + (at + i) * D + 4 * c);
-    if constexpr (GROUPS > 1) {
-        sums[threadIdx.x] = x;
-        __syncthreads();
-        if (grp > 0) return;
-#pragma unroll
-        for (int i = 1; i < GROUPS; ++i) x += sums[i * TC + c];
+        for (int i = first; i - first < count; i += step) {
+            const int one = min(i, count - 1);
+            const float w = __shfl(weight, one);
+            const f4 part = *(const f4*)(p.po + (at + from + one) * D + col);
+            if (i < count) x += w * part;
+        }
     }
-    if (grp > 0) return;
-    Piece4<T> y;
+    sum = wave_sum(sum);
+    if (s.bad) sum = NAN;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y.e[e] = (T)(x[e] / total[0]);
-    *(Piece4<T>*)((T*)p.out + t * p.os + (long long)head * D + 4 * c) = y;
+    for (int o = LANES; o < kWave; o *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], o);
+    if (together) {
+        if (wave > 0 && lane < LANES) sums[wave - 1][lane] = x;
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 0; w + 1 < kWaves; ++w) x += sums[w][lane % LANES];
+    }
+    if (lane < LANES) {
+        Piece4<T> y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y.e[e] = (T)(x[e] / sum);
+        *(Piece4<T>*)((T*)p.out + t * p.os + (long long)head * D + col) = y;
+    }
 }
 
 // --------------------------------------------------------------------------
@@ -935,18 +992,21 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(AttendParams p, int pr
 struct Range {
     int splits, chunk;
 };
+constexpr int kMaxSplits = 256;
 
-// Ranges that `keys` keys are divided into where there are `items` items of all
-// of them: enough for `want` workgroups, each at least a tile of every
-// wavefront.
-static Range ranges(long long items, int keys, int step, int most) {
-    const long long want = 4LL * device_cu_count();
-    long long s = items > 0 ? want / items : 1;
-    s = std::min<long long>(s, keys / step);
-    s = std::max<long long>(1, std::min<long long>(s, most));
+// Ranges that `keys` keys are divided into where all of them are `items` items of
+// work: as many as make `want` workgroups, each of `step` keys or more; with
+// several row tiles to a range, of a number that lets the streams deal onto
+// the XCDs (find_item).
+static Range ranges(long long items, int keys, int step, long long want, int kv, bool single) {
+    long long s = std::min<long long>(items > 0 ? want / items : 1, keys / step);
+    s = std::max<long long>(1, std::min<long long>(s, kMaxSplits));
+    int deal = kNumXcd;
+    while (deal > 1 && (long long)kv * deal / 2 % kNumXcd == 0) deal /= 2;
+    if (!single && s > deal) s -= s % deal;
     long long chunk = (keys + s - 1) / s;
     chunk = std::max<long long>(step, (chunk + step - 1) / step * step);
-    return {(int)std::max<long long>(1, (keys + chunk - 1) / chunk), (int)chunk};
+    return {single ? (int)std::max<long long>(1, (keys + chunk - 1) / chunk) : (int)s, (int)chunk};
 }
 
 struct Plan {
@@ -955,6 +1015,9 @@ struct Plan {
     int tiles, prefix_tiles;
     Range own, prefix;
     int slots() const { return own.splits + prefix.splits; }
+    int prefix_parts(int len) const {
+        return std::min(prefix.splits, (int)((len + (long long)prefix.chunk - 1) / prefix.chunk));
+    }
 };
 
 static int tile_rows(int dim) { return dim > 128 ? TileShape<256>::kRows : TileShape<128>::kRows; }
@@ -962,21 +1025,24 @@ static int tile_rows(int dim) { return dim > 128 ? TileShape<256>::kRows : TileS
 static Plan plan(const Attention& a) {
     Plan p;
     const int kv = (int)a.pages.kv_heads, group = a.heads / kv, dim = a.pages.dim;
-    const bool tiled = a.dtype != XATTN_F32 && dim <= 256;  // cache_tile_kernel takes it
+    const bool tiled = a.dtype != XATTN_F32 && dim <= 256;  // tile_item takes it
     const int few = (a.dtype == XATTN_F32 ? 16 : 32) * (dim > 256 ? 1 : kWaves);
     const int many = dim > 128 ? TileShape<256>::kKeys : TileShape<128>::kKeys;
     const long long rows = (long long)a.batch.tokens * group, most = (long long)a.max_q * group;
+    const long long cu = device_cu_count();
     p.single = most <= kRows;
     p.rows = tiled && most > kManyRows ? tile_rows(dim) : kRows;
     p.tiles = p.single ? a.batch.batch
                        : (int)std::min<long long>(rows / p.rows + a.batch.batch,
                                                   (most + p.rows - 1) / p.rows * a.batch.batch);
-    p.own = ranges((long long)p.tiles * kv, a.max_kv, p.rows > kRows ? many : few, kMaxSlots / 2);
+    p.own = ranges((long long)p.tiles * kv, a.max_kv, p.rows > kRows ? TILE_STEP * many : few,
+                   p.single ? WANT_SINGLE * cu : p.rows > kRows ? WANT_TILE * cu : WANT_FEW * cu, kv, p.single);
     p.prefix_rows = tiled && rows > kManyRows ? tile_rows(dim) : kRows;
     p.prefix_tiles = (int)((rows + p.prefix_rows - 1) / p.prefix_rows);
-    p.prefix = a.prefix_len > 0 ? ranges((long long)p.prefix_tiles * kv, a.prefix_len,
-                                         p.prefix_rows > kRows ? many : few, kMaxSlots / 2)
-                                : Range{0, 1};
+    p.prefix = a.prefix_len > 0
+                   ? ranges((long long)p.prefix_tiles * kv, a.prefix_len,
+                            p.prefix_rows > kRows ? TILE_STEP * many : few, WANT_PREFIX * cu, kv, false)
+                   : Range{0, 1};
     return p;
 }
 
@@ -989,32 +1055,41 @@ size_t attention_scratch(const Attention& a) {
     return parts(a, plan(a)) * (a.pages.dim * sizeof(float) + sizeof(float2));
 }
 
-template <typename T, int D, bool PREFIX>
-static void attend(const AttendParams& p, int rows, hipStream_t stream) {
-    const unsigned grid = p.pages.kv_heads * (unsigned)p.tiles * (unsigned)p.splits;
-    if constexpr (sizeof(T) == 2 && D <= 256)
-        if (rows > kRows) {
-            cache_tile_kernel<T, D, PREFIX><<<grid, 256, 0, stream>>>(p);
-            return;
-        }
-    cache_attend_kernel<T, D, PREFIX><<<grid, 256, 0, stream>>>(p);
+static unsigned blocks(const AttendParams& p) {
+    return p.pages.kv_heads * (unsigned)p.tiles * (unsigned)p.splits;
 }
 
 template <typename T, int D>
-static void go(AttendParams& p, const Plan& plan, hipStream_t stream) {
+static void go(const AttendParams& own, const Plan& plan, hipStream_t stream) {
+    constexpr bool tiled = sizeof(T) == 2 && D <= 256;
+    const bool tile = tiled && plan.rows > kRows, prefix_tile = tiled && plan.prefix_rows > kRows;
     if (plan.prefix.splits > 0) {
-        AttendParams f = p;
-        f.single = 0;
-        f.tiles = plan.prefix_tiles;
-        f.splits = plan.prefix.splits;
-        f.chunk = plan.prefix.chunk;
-        f.slot = 0;
-        attend<T, D, true>(f, plan.prefix_rows, stream);
+        AttendParams p = own;
+        p.single = 0;
+        p.tiles = plan.prefix_tiles;
+        p.splits = plan.prefix.splits;
+        p.chunk = plan.prefix.chunk;
+        p.slot = 0;
+        const unsigned first = blocks(p), all = first + blocks(own);
+        if constexpr (tiled) {
+            if (tile)
+                cache_prefix_kernel<T, D, 2><<<all, 256, 0, stream>>>(p, own, first);
+            else if (prefix_tile)
+                cache_prefix_kernel<T, D, 1><<<all, 256, 0, stream>>>(p, own, first);
+        }
+        if (!prefix_tile) cache_prefix_kernel<T, D, 0><<<all, 256, 0, stream>>>(p, own, first);
+    } else if (tile) {
+        if constexpr (tiled) cache_tile_kernel<T, D><<<blocks(own), 256, 0, stream>>>(own);
+    } else {
+        cache_attend_kernel<T, D><<<blocks(own), 256, 0, stream>>>(own);
     }
-    attend<T, D, false>(p, plan.rows, stream);
-    if (p.po)
-        cache_merge_kernel<T, D><<<(unsigned)p.batch.tokens * p.heads, 256, 0, stream>>>(
-            p, plan.prefix.splits);
+    if (own.po) {
+        const long long units = (long long)own.batch.tokens * own.heads * (D > 256 ? D / 256 : 1);
+        const bool together = units < 8 * device_cu_count();
+        cache_merge_kernel<T, D>
+            <<<(unsigned)(together ? units : (units + kWaves - 1) / kWaves), 256, 0, stream>>>(
+                own, own.slot, together);
+    }
 }
 
 template <typename T>
@@ -1048,7 +1123,7 @@ bool launch_attention(const Attention& a, void* scratch, hipStream_t stream) {
     p.single = pl.single;
     p.splits = pl.own.splits;
     p.chunk = pl.own.chunk;
-    p.slot = pl.prefix.splits;
+    p.slot = pl.prefix_parts(a.prefix_len);
     p.slots = pl.slots();
     if (const size_t n = parts(a, pl)) {
         p.po = (float*)scratch;
