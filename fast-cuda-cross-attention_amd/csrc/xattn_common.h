@@ -95,6 +95,13 @@ __device__ inline void wait_vmcnt() {
     compiler_fence();
 }
 
+// Waits for this wave's own LDS operations, and leaves the others in flight.
+__device__ inline void wait_lds() {
+    compiler_fence();
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), vmcnt/expcnt unconstrained
+    compiler_fence();
+}
+
 // Workgroup barrier for LDS hand-off: waits for this wave's own LDS
 // operations, then s_barrier.  Unlike __syncthreads() it carries no release
 // fence, so global->LDS DMA issued for later phases stays in flight; the
