@@ -16,9 +16,13 @@
 // row r of block b); in 16 bits they pass through LDS to be read transposed.
 //
 // A tile's scores come before the product of the tile before it with V, under which
-// the next K is asked for and the shares of the scores are exchanged; then V of
-// this tile is asked for, and its softmax done.  So everything that arrives has a
-// product's time to do so, and a K and a V of each wavefront are enough.
+// the shares of the scores are exchanged; its softmax comes last.  What the next
+// steps need is asked for piece by piece between the matrix instructions (in one
+// run it would hold the wavefront until the path to memory has taken it, 968 cycles
+// for V at 768 columns in 32 bits): in 32 bits the next K under the scores, into the
+// other of two slots, and this tile's V under the product, register by register as
+// the old ones have been used; in 16 bits, whose LDS has room for one K only, the
+// next K under the product and V behind it.
 #pragma once
 
 #include "xattn_cache_item.h"
@@ -41,12 +45,14 @@ struct RingShape {
         64 % kPieces == 0 ? 1 : kPieces % 16 == 0 ? kPieces / 16 : kPieces / 8;
     static constexpr int kStep = 64 * kPeriod / kPieces;
     static constexpr int kKTile = kRegs * 1024;
+    static constexpr int kSlots = kWide ? 2 : 1;        // K tiles of a wavefront in LDS
     static constexpr int kVRow = kRow + 32;             // in LDS; 32 bytes of padding deal four
                                                         // rows to distinct banks
     static constexpr int kVTile = kWide ? 0 : kKeys * kVRow;
     static constexpr int kORow = kDW + 4;               // floats of an output row in LDS
     static constexpr int kOut = kCols > 1 ? 0 : kRows * kORow * 4;
-    static constexpr int kWaveLds = kKTile + kVTile > kOut ? kKTile + kVTile : kOut;
+    static constexpr int kTiles = kSlots * kKTile + kVTile;
+    static constexpr int kWaveLds = kTiles > kOut ? kTiles : kOut;
     static constexpr int kShare = kKeys * kRows * 4;    // bytes of a wavefront's share of scores
     static constexpr int kShares = kCols > 1 ? 2 * kWaves * kShare : 0;
     static constexpr int kStats = kWaves * kRows * 8;   // maxima and sums
@@ -128,10 +134,11 @@ __device__ __forceinline__ void ring_item(const AttendParams& p, unsigned block,
         const int row = STEP * (c / PERIOD) + k_row[c % PERIOD];
         return 16 * (k_piece[c % PERIOD] ^ S::swizzle(row));
     };
-    const auto dma_whole = [&](const DmaSrc (&from)[KB], int c) {
+    const auto dma_whole = [&](const DmaSrc (&from)[KB], int slot, int c) {
         const int row = STEP * (c / PERIOD);
         dma16_m0<0>(from[row / 16] + (size_t)(row % 16 * ROW),
-                    (unsigned)(k_row[c % PERIOD] * ROW + k_from(c)), kt_at + 1024 * c);
+                    (unsigned)(k_row[c % PERIOD] * ROW + k_from(c)),
+                    kt_at + slot * S::kKTile + 1024 * c);
     };
     DmaSrc pool;
     {
@@ -143,58 +150,55 @@ __device__ __forceinline__ void ring_item(const AttendParams& p, unsigned block,
         for (int h = 0; h < KB; ++h)
             from[h] = pool + (size_t)(half(p.pages.k, ids, k, h) - p.pages.k);
     };
-    const auto dma_any = [&](int ids, int k) {
+    const auto dma_any = [&](int ids, int k, int slot) {
 #pragma unroll
         for (int c = 0; c < NR; ++c)
             dma16_lanes(one(p.pages.k, ids, k, STEP * (c / PERIOD) + k_row[c % PERIOD]) + k_from(c),
-                        kt_at + 1024 * c);
+                        kt_at + slot * S::kKTile + 1024 * c);
     };
 
     // V in registers.  32 bits: register r is columns 64 (r / 4) + 4 j on of row 4 g +
     // r % 4.  16 bits: KiB r in row order.
     u4 vr[NR];
-    const auto load_v = [&](int ids, int k) {
-        if (runs && k + KT <= k1) {
-            const char* from[KB];
+    const auto v_whole = [&](int ids, int k, const char* (&from)[KB]) {
 #pragma unroll
-            for (int h = 0; h < KB; ++h) from[h] = half(p.pages.v, ids, k, h);
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                if constexpr (WIDE) {
-                    const unsigned at = 4 * g * ROW + 16 * j;
-                    vr[r] = *(const u4*)(from[0] + (r % 4 * ROW + 256 * (r / 4)) + at);
-                } else {
-                    const int row = STEP * (r / PERIOD);
-                    const unsigned at = k_row[r % PERIOD] * ROW + 16 * k_piece[r % PERIOD];
-                    vr[r] = *(const u4*)(from[row / 16] + row % 16 * ROW + at);
-                }
-            }
+        for (int h = 0; h < KB; ++h) from[h] = half(p.pages.v, ids, k, h);
+    };
+    const auto load_whole = [&](const char* const (&from)[KB], int r) {
+        if constexpr (WIDE) {
+            const unsigned at = 4 * g * ROW + 16 * j;
+            vr[r] = *(const u4*)(from[0] + (r % 4 * ROW + 256 * (r / 4)) + at);
         } else {
+            const int row = STEP * (r / PERIOD);
+            const unsigned at = k_row[r % PERIOD] * ROW + 16 * k_piece[r % PERIOD];
+            vr[r] = *(const u4*)(from[row / 16] + row % 16 * ROW + at);
+        }
+    };
+    const auto load_any = [&](int ids, int k) {
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                if constexpr (WIDE)
-                    vr[r] = *(const u4*)(one(p.pages.v, ids, k, 4 * g + r % 4) + 256 * (r / 4) +
-                                         16 * j);
-                else
-                    vr[r] = *(const u4*)(one(p.pages.v, ids, k,
-                                             STEP * (r / PERIOD) + k_row[r % PERIOD]) +
-                                         16 * k_piece[r % PERIOD]);
-            }
+        for (int r = 0; r < NR; ++r) {
+            if constexpr (WIDE)
+                vr[r] = *(const u4*)(one(p.pages.v, ids, k, 4 * g + r % 4) + 256 * (r / 4) + 16 * j);
+            else
+                vr[r] = *(const u4*)(one(p.pages.v, ids, k,
+                                         STEP * (r / PERIOD) + k_row[r % PERIOD]) +
+                                     16 * k_piece[r % PERIOD]);
         }
     };
 
-    // The product of the weights `w` with the V in registers; between its steps, `also`.
-    char* const vt = kt + S::kKTile;
+    // The product of the weights `w` with the V in registers.  Between its steps comes
+    // also(r); in 32 bits V's register r is free by then.
+    char* const vt = kt + S::kSlots * S::kKTile;
     f4 w[KB];
     const auto product = [&](auto also) {
         if constexpr (WIDE) {
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                also(r);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     o[r / 4 * 4 + e] =
                         mfma4(__uint_as_float(vr[r][e]), w[0][r % 4], o[r / 4 * 4 + e]);
+                also(r);
             }
         } else {
 #pragma unroll
@@ -216,26 +220,38 @@ __device__ __forceinline__ void ring_item(const AttendParams& p, unsigned block,
     int k = k0 + (SHARED ? 0 : wave * KT);
     if (k < k1) {
         int ids = find(k), ids1 = find(k + step);
-        dma_any(ids, k);
+        dma_any(ids, k, 0);
         wait_vmcnt<0>();
         bool first = true, partial = false;
         for (int turn = 0; k < k1; k += step, turn ^= 1) {
-            const bool more = k + step < k1;
+            const bool more = k + step < k1, whole = runs && k + KT <= k1;
+            const bool whole1 = more && runs && k + step + KT <= k1;
             const int ids2 = find(k + 2 * step);
-            // Scores; in 32 bits in four sums, as a product takes longer to come out
-            // than to start.
             f4 sc[KB];
             if constexpr (WIDE) {
-                f4 part[4];
+                // in four sums, as a product takes longer to come out than to start
+                const char* const from = kt + turn * S::kKTile + j * S::kRow;
+                const auto scores = [&](auto also) {
+                    f4 part[4];
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    const u4 a = *(const u4*)(kt + j * S::kRow + 16 * (4 * r + g ^ S::swizzle(j)));
+                    for (int r = 0; r < NR; ++r) {
+                        const u4 a = *(const u4*)(from + 16 * (4 * r + g ^ S::swizzle(j)));
+                        also(r);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        part[e] = mfma4(__uint_as_float(a[e]), __uint_as_float(qr[r][e]),
-                                        r ? part[e] : f4{0, 0, 0, 0});
+                        for (int e = 0; e < 4; ++e)
+                            part[e] = mfma4(__uint_as_float(a[e]), __uint_as_float(qr[r][e]),
+                                            r ? part[e] : f4{0, 0, 0, 0});
+                    }
+                    sc[0] = (part[0] + part[1]) + (part[2] + part[3]);
+                };
+                if (whole1) {
+                    DmaSrc next[KB];
+                    k_whole(ids1, k + step, next);
+                    scores([&](int r) { dma_whole(next, turn ^ 1, r); });
+                } else {
+                    if (more) dma_any(ids1, k + step, turn ^ 1);
+                    scores([](int) {});
                 }
-                sc[0] = (part[0] + part[1]) + (part[2] + part[3]);
             } else {
 #pragma unroll
                 for (int r = 0; r < NQ; ++r)
@@ -251,7 +267,7 @@ __device__ __forceinline__ void ring_item(const AttendParams& p, unsigned block,
 #pragma unroll
                 for (int h = 0; h < KB; ++h)
                     *(f4*)(share + wave * S::kShare + (h * kWave + lane) * 16) = sc[h];
-            // The tile before: its product, and under it the next K and the barrier.
+            // The product of the tile before.
             if (!first && partial)
 #pragma unroll
                 for (int r = 0; r < NR; ++r) odd |= clear_not_finite<T>(vr[r]);
@@ -259,22 +275,46 @@ __device__ __forceinline__ void ring_item(const AttendParams& p, unsigned block,
                 if constexpr (SHARED)
                     if (r == NR / 2) lds_barrier();
             };
-            if (more) wait_lds();  // this K has been read
-            if (!first && more && runs && k + step + KT <= k1) {
-                DmaSrc from[KB];
-                k_whole(ids1, k + step, from);
-                product([&](int r) {
-                    dma_whole(from, r);
-                    meet(r);
-                });
+            if constexpr (WIDE) {
+                if (!first && whole) {
+                    const char* from[KB];
+                    v_whole(ids, k, from);
+                    product([&](int r) {
+                        load_whole(from, r);
+                        meet(r);
+                    });
+                } else {
+                    if (first)
+                        meet(NR / 2);
+                    else
+                        product(meet);
+                    load_any(ids, k);
+                }
             } else {
-                if (more) dma_any(ids1, k + step);
-                if (first)
-                    meet(NR / 2);
-                else
-                    product(meet);
+                if (more) wait_lds();  // this K has been read
+                if (!first && whole1) {
+                    DmaSrc next[KB];
+                    k_whole(ids1, k + step, next);
+                    product([&](int r) {
+                        dma_whole(next, 0, r);
+                        meet(r);
+                    });
+                } else {
+                    if (more) dma_any(ids1, k + step, 0);
+                    if (first)
+                        meet(NR / 2);
+                    else
+                        product(meet);
+                }
+                if (whole) {
+                    const char* from[KB];
+                    v_whole(ids, k, from);
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) load_whole(from, r);
+                } else {
+                    load_any(ids, k);
+                }
             }
-            load_v(ids, k);
             if constexpr (SHARED)
 #pragma unroll
                 for (int h = 0; h < KB; ++h) {
@@ -293,7 +333,7 @@ __device__ __forceinline__ void ring_item(const AttendParams& p, unsigned block,
             first = false;
             ids = ids1;
             ids1 = ids2;
-            // The next K has arrived: it was asked for before the NR loads of V.
+            // The next K has arrived: it was asked for before the NR loads of this V.
             if (more) wait_vmcnt<NR>();
         }
         if (partial)
