@@ -50,7 +50,17 @@ struct Rope {
     bool interleaved, inverse;
 };
 
-constexpr int kMaxRot = 2048;  // rotated elements of a head: their angles fit LDS
+constexpr int kMaxRot = 2048;          // rotated elements of a head: their angles fit LDS
+constexpr int kMaxKeys = 1 << 30;      // of a sequence or prefix: sums of positions fit an int
+constexpr int kMaxBlocks = 0xffffff;   // workgroups of 256 threads in a launch
+
+// Whether a launch of this many workgroups is possible; records the error if not.
+inline bool grid_fits(const char* who, long long blocks) {
+    if (blocks <= kMaxBlocks) return true;
+    set_error(XATTN_ERR_UNSUPPORTED, "%s: a call of %lld workgroups, over %d", who, blocks,
+              kMaxBlocks);
+    return false;
+}
 
 // Launchers; the arguments are valid (xattn_cache_abi.h).
 bool launch_rope(const void* x, void* y, const int* positions, const Rope& rope, int dtype,

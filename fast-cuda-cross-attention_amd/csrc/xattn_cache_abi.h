@@ -109,6 +109,10 @@ static bool view_batch(const char* who, const xattn_batch* b, int page_size, boo
         return refuse(who, "NULL q_starts, kv_lens or page_table");
     if (((uintptr_t)b->q_starts | (uintptr_t)b->kv_lens | (uintptr_t)b->page_table) % 4 != 0)
         return refuse(who, "q_starts, kv_lens or page_table is not 4-byte aligned");
+    if ((long long)b->table_width * page_size > kMaxKeys) {
+        set_error(XATTN_ERR_UNSUPPORTED, "%s: rows of page_table for over 2^30 keys", who);
+        return false;
+    }
     *out = Batch{b->q_starts, b->kv_lens, b->page_table, b->batch, b->table_width, b->tokens,
                  (long long)b->table_width * page_size};
     return true;
@@ -142,6 +146,10 @@ static bool view_attention(const char* who, const xattn_kv_cache* cache, const x
             (long long)prefix->num_listed * cache->page_size < prefix->len) {
             set_error(XATTN_ERR_INVALID_VALUE, "%s: a prefix of %d keys on %d pages of %d", who,
                       prefix->len, prefix->num_listed, cache->page_size);
+            return false;
+        }
+        if (prefix->len > kMaxKeys) {
+            set_error(XATTN_ERR_UNSUPPORTED, "%s: a prefix of over 2^30 keys", who);
             return false;
         }
         if (!sizes_only && prefix->len > 0 && !prefix->pages)

@@ -5,7 +5,8 @@
 // The query heads of one kv head see the same keys, so a sequence's rows are
 // its (token, head of the group) pairs, `group` to a token.  A work item is
 // (kv head, a tile of rows, a range of keys) on one workgroup of four wavefronts, in
-// one of three forms: xattn_cache_few.h, xattn_cache_ring.h, xattn_cache_tile.h.
+// one of four forms: xattn_cache_few.h and xattn_cache_tile.h (16 bits up to dim 256),
+// xattn_cache_ring.h (16 bits at 768), xattn_cache_wide.h (32 bits).
 // Where there are fewer items than the device needs, the keys are divided and a
 // second launch merges the parts.  For the prefix the rows are those of the whole
 // batch, so that its keys are read once for a tile of rows of any sequences.
@@ -17,75 +18,79 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "xattn_cache_few.h"
 #include "xattn_cache_ring.h"
 #include "xattn_cache_tile.h"
+#include "xattn_cache_wide.h"
 #include "xattn_launch.h"
 
 namespace xattn {
 namespace cache {
 
-#ifndef WANT_TILE
-#define WANT_TILE 6
-#define WANT_FEW 1
-#define WANT_SINGLE 8
-#define WANT_PREFIX 1
-#define TILE_STEP 2
-#endif
 // --------------------------------------------------------------------------
 // Kernels.  The keys of a prefix and those of the sequences are worked on in
 // one launch, the prefix's (longer) items first: the sequences' fill in.
 // --------------------------------------------------------------------------
-// Which form takes a few rows: attend_item in 16 bits up to dim 256, else ring_item.
-template <typename T, int D>
-constexpr bool kRing = sizeof(T) == 4 || D > 256;
-template <typename T, int D>
-constexpr int few_lds() {
-    if constexpr (kRing<T, D>)
-        return RingShape<T, D>::kLds;
-    else
-        return FewShape<T, D>::kLds;
-}
-template <typename T, int D, bool PREFIX>
-__device__ __forceinline__ void few_item(const AttendParams& p, unsigned block, char* lds) {
-    if constexpr (kRing<T, D>)
-        ring_item<T, D, PREFIX>(p, block, lds);
-    else
-        attend_item<T, D, PREFIX>(p, block, lds);
-}
 
+// The forms by type and dim: that of a few rows (one block of sixteen), and that of
+// many.  In 32 bits two blocks pay at 128 only: 1,024 tokens over 1,500 keys took
+// 101 us with two and 120 with one there, but 69 and 62 at 64, 158 and 122 at 256, 79
+// and 66 (512 tokens) at 768, where two leave too few registers or workgroups.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void cache_attend_kernel(AttendParams p) {
-    __shared__ __align__(16) char lds[few_lds<T, D>()];
-    few_item<T, D, false>(p, blockIdx.x, lds);
-}
-
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void cache_tile_kernel(AttendParams p) {
-    __shared__ __align__(16) char lds[TileShape<D>::kLds];
-    tile_item<T, D, false>(p, blockIdx.x, lds);
-}
-
-// TILES: how many of the two go by tile_item (2: both, 1: the prefix, 0: none).
-template <typename T, int D, int TILES>
-__global__ __launch_bounds__(256, TILES == 2 || (TILES == 1 && D <= 128) ? 2 : 1) void
-cache_prefix_kernel(
-    AttendParams prefix, AttendParams own, unsigned prefix_blocks) {
-    constexpr int few = TILES < 2 ? few_lds<T, D>() : 0;
-    constexpr int many = TILES > 0 ? TileShape<D>::kLds : 0;
-    __shared__ __align__(16) char lds[few > many ? few : many];
-    if (blockIdx.x < prefix_blocks) {
-        if constexpr (TILES > 0)
-            tile_item<T, D, true>(prefix, blockIdx.x, lds);
+struct Forms {
+    static constexpr bool kWide = sizeof(T) == 4, kRing = !kWide && D > 256;
+    static constexpr bool kMany = !kWide || D == 128;
+    // Rows of a work item of many, and the rows of a sequence from which on it is taken.
+    static constexpr int kHeight = kWide || kRing ? 2 * kRows : TileShape<D>::kRows;
+    static constexpr int kFrom = kWide || kRing ? kRows + 1 : 2 * kRows + 1;
+    // Keys of a tile of the two, over all wavefronts.
+    static constexpr int kFewKeys = kWide  ? WideShape<D, 1>::kKeys * kWaves / WideShape<D, 1>::kCols
+                                    : kRing ? RingShape<1>::kKeys
+                                            : FewShape<T, D>::kKeys * kWaves;
+    static constexpr int kManyKeys = kWide || kRing ? kFewKeys : TileShape<D>::kKeys;
+    static constexpr int lds(bool many) {
+        if constexpr (kWide)
+            return many ? WideShape<D, 2>::kLds : WideShape<D, 1>::kLds;
+        else if constexpr (kRing)
+            return many ? RingShape<2>::kLds : RingShape<1>::kLds;
         else
-            few_item<T, D, true>(prefix, blockIdx.x, lds);
-    } else {
-        if constexpr (TILES > 1)
-            tile_item<T, D, false>(own, blockIdx.x - prefix_blocks, lds);
-        else
-            few_item<T, D, false>(own, blockIdx.x - prefix_blocks, lds);
+            return many ? TileShape<D>::kLds : FewShape<T, D>::kLds;
     }
+    static constexpr int max_lds(bool a, bool b) { return lds(a) > lds(b) ? lds(a) : lds(b); }
+    // Wavefronts that a SIMD has to hold: two of tile_item, in 256 registers each.
+    static constexpr int waves(bool many) { return !kWide && !kRing && many ? 2 : 1; }
+    template <bool MANY, bool PREFIX>
+    static __device__ __forceinline__ void item(const AttendParams& p, unsigned block, char* lds) {
+        if constexpr (kWide)
+            wide_item<D, MANY ? 2 : 1, PREFIX>(p, block, lds);
+        else if constexpr (kRing)
+            ring_item<T, MANY ? 2 : 1, PREFIX>(p, block, lds);
+        else if constexpr (MANY)
+            tile_item<T, D, PREFIX>(p, block, lds);
+        else
+            attend_item<T, D, PREFIX>(p, block, lds);
+    }
+};
+
+template <typename T, int D, bool MANY>
+__global__ __launch_bounds__(256, (Forms<T, D>::waves(MANY))) void
+cache_attend_kernel(AttendParams p) {
+    __shared__ __align__(16) char lds[Forms<T, D>::lds(MANY)];
+    Forms<T, D>::template item<MANY, false>(p, blockIdx.x, lds);
+}
+
+// PREFIX_MANY, MANY: the forms of the prefix's items and of the sequences'.
+template <typename T, int D, bool PREFIX_MANY, bool MANY>
+__global__ __launch_bounds__(256, (PREFIX_MANY && (MANY || D <= 128) ? Forms<T, D>::waves(true)
+                                                                     : 1)) void
+cache_prefix_kernel(AttendParams prefix, AttendParams own, unsigned prefix_blocks) {
+    __shared__ __align__(16) char lds[Forms<T, D>::max_lds(PREFIX_MANY, MANY)];
+    if (blockIdx.x < prefix_blocks)
+        Forms<T, D>::template item<PREFIX_MANY, true>(prefix, blockIdx.x, lds);
+    else
+        Forms<T, D>::template item<MANY, false>(own, blockIdx.x - prefix_blocks, lds);
 }
 
 // --------------------------------------------------------------------------
@@ -166,27 +171,27 @@ struct Range {
     int splits, chunk;
 };
 constexpr int kMaxSplits = 256;
-constexpr int kManyRows = 32;  // rows of a sequence beyond which tile_item takes it
 
-// Ranges that `keys` keys are divided into where all of them are `items` items of
-// work: as many as make `want` workgroups, each of `step` keys or more; with
-// several row tiles to a range, of a number that lets the streams deal onto
-// the XCDs (find_item).
-static Range ranges(long long items, int keys, int step, long long want, int kv, bool single) {
-    long long s = std::min<long long>(items > 0 ? want / items : 1, keys / step);
+// `keys` keys in about `s` ranges, each of `step` keys or more.  `deal`: of a number
+// that lets the streams of kv kv heads deal onto the XCDs (find_item).
+static Range ranges(long long s, int keys, int step, int kv, bool deal) {
+    s = std::min<long long>(s, keys / step);
     s = std::max<long long>(1, std::min<long long>(s, kMaxSplits));
-    int deal = kNumXcd;
-    while (deal > 1 && (long long)kv * deal / 2 % kNumXcd == 0) deal /= 2;
-    if (!single && s > deal) s -= s % deal;
+    if (deal) {
+        int by = kNumXcd;
+        while (by > 1 && (long long)kv * by / 2 % kNumXcd == 0) by /= 2;
+        if (s > by) s -= s % by;
+    }
     long long chunk = (keys + s - 1) / s;
     chunk = std::max<long long>(step, (chunk + step - 1) / step * step);
-    return {single ? (int)std::max<long long>(1, (keys + chunk - 1) / chunk) : (int)s, (int)chunk};
+    if (!deal) s = std::max<long long>(1, (keys + chunk - 1) / chunk);
+    return {(int)s, (int)chunk};
 }
 
 struct Plan {
-    bool single;            // every sequence has at most sixteen rows
-    int rows, prefix_rows;  // rows of a work item
-    int tiles, prefix_tiles;
+    bool single;                 // every sequence has one row tile
+    bool many, prefix_many;      // the forms
+    int tiles, prefix_tiles;     // row tiles
     Range own, prefix;
     int slots() const { return own.splits + prefix.splits; }
     int prefix_parts(int len) const {
@@ -194,29 +199,56 @@ struct Plan {
     }
 };
 
-static int tile_rows(int dim) { return dim > 128 ? TileShape<256>::kRows : TileShape<128>::kRows; }
-
+// How often the keys are divided.
+//   One row tile to a sequence: enough for a workgroup a CU, and so that none has
+// more than 1 MiB of K and V to read (3 at dim 768, where a workgroup has a CU to
+// itself), as sequences may be of unlike lengths: 64 of up to 8,192 keys, 8 kv heads
+// of 128, take 214 us in ranges of 1 MiB, 232 in ranges of 2.  Up to 256 KiB stay
+// whole even on an idle device: 784 keys of 64 take 9.7 us whole and 13.4 in seven
+// parts with the merge, 3,000 take 20.8 and 12.6.
+//   Several row tiles: a workgroup a CU; of tile_item four, against unlike lengths
+// (six prompt pieces of 106 .. 700 tokens, kv heads of 64: 83 us with two, 75 with
+// four and ten; a prompt of 4,096, heads of 128: 153 with two and four, 196 with ten).
+//   The prefix: a workgroup a CU (32 tokens over 16,384 keys, 8 kv heads of 128: 37
+// us, 46 with two, 50 with three: more parts to merge).
+template <typename T, int D>
 static Plan plan(const Attention& a) {
+    typedef Forms<T, D> F;
+    constexpr long long row = 2LL * D * sizeof(T);  // bytes of a key and its value
     Plan p;
-    const int kv = (int)a.pages.kv_heads, group = a.heads / kv, dim = a.pages.dim;
-    const bool tiled = a.dtype != XATTN_F32 && dim <= 256;  // tile_item takes it
-    const int few = (a.dtype == XATTN_F32 ? 16 : 32) * (dim > 256 ? 1 : kWaves);
-    const int many = dim > 128 ? TileShape<256>::kKeys : TileShape<128>::kKeys;
+    const int kv = (int)a.pages.kv_heads, group = a.heads / kv;
     const long long rows = (long long)a.batch.tokens * group, most = (long long)a.max_q * group;
     const long long cu = device_cu_count();
-    p.single = most <= kRows;
-    p.rows = tiled && most > kManyRows ? tile_rows(dim) : kRows;
+    constexpr bool tile = !F::kWide && !F::kRing;
+    // Two blocks instead of one pay where a CU has many keys to pass them by, as every
+    // range has a start and a tail: in 16 bits at 768, 64 rows over 16,000 keys take 42
+    // us with two and 36 with one, over 50,176 keys 69 and 79; in 32 bits at 128, 256
+    // rows of 8 kv heads over 784 keys 25 and 22, 2,048 over 1,500 keys 101 and 119.
+    const long long passes = std::min(rows / kRows + a.batch.batch,
+                                      (most + kRows - 1) / kRows * a.batch.batch) * a.max_kv +
+                             rows / kRows * a.prefix_len;
+    const bool enough = tile || passes * kv >= (F::kRing ? 512 : 1024) * cu;
+    p.many = F::kMany && enough && most >= F::kFrom;
+    const int height = p.many ? F::kHeight : kRows;
+    p.single = most <= height;
     p.tiles = p.single ? a.batch.batch
-                       : (int)std::min<long long>(rows / p.rows + a.batch.batch,
-                                                  (most + p.rows - 1) / p.rows * a.batch.batch);
-    p.own = ranges((long long)p.tiles * kv, a.max_kv, p.rows > kRows ? TILE_STEP * many : few,
-                   p.single ? WANT_SINGLE * cu : p.rows > kRows ? WANT_TILE * cu : WANT_FEW * cu, kv, p.single);
-    p.prefix_rows = tiled && rows > kManyRows ? tile_rows(dim) : kRows;
-    p.prefix_tiles = (int)((rows + p.prefix_rows - 1) / p.prefix_rows);
-    p.prefix = a.prefix_len > 0
-                   ? ranges((long long)p.prefix_tiles * kv, a.prefix_len,
-                            p.prefix_rows > kRows ? TILE_STEP * many : few, WANT_PREFIX * cu, kv, false)
-                   : Range{0, 1};
+                       : (int)std::min<long long>(rows / height + a.batch.batch,
+                                                  (most + height - 1) / height * a.batch.batch);
+    const long long items = std::max<long long>(1, (long long)p.tiles * kv);
+    long long s = (tile && p.many && !p.single ? 4 : 1) * cu / items;
+    if (p.single) {
+        const long long by_size = a.max_kv * row / ((D > 256 ? 3LL : 1LL) << 20);
+        s = std::max(s, std::min(by_size, 16 * cu / items));
+        if (a.max_kv * row <= 256 << 10) s = 1;
+    }
+    p.own = ranges(s, a.max_kv, tile && p.many ? 2 * F::kManyKeys : F::kFewKeys, kv, !p.single);
+    p.prefix_many = F::kMany && enough && rows >= F::kFrom;
+    const int prefix_height = p.prefix_many ? F::kHeight : kRows;
+    p.prefix_tiles = (int)((rows + prefix_height - 1) / prefix_height);
+    p.prefix = Range{0, 1};
+    if (a.prefix_len > 0)
+        p.prefix = ranges(cu / std::max<long long>(1, (long long)p.prefix_tiles * kv),
+                          a.prefix_len, tile && p.prefix_many ? 2 * F::kManyKeys : F::kFewKeys, kv, true);
     return p;
 }
 
@@ -225,88 +257,101 @@ static size_t parts(const Attention& a, const Plan& p) {
     return (size_t)a.batch.tokens * a.heads * p.slots();
 }
 
-size_t attention_scratch(const Attention& a) {
-    return parts(a, plan(a)) * (a.pages.dim * sizeof(float) + sizeof(float2));
-}
-
-static unsigned blocks(const AttendParams& p) {
-    return p.pages.kv_heads * (unsigned)p.tiles * (unsigned)p.splits;
+static long long blocks(const AttendParams& p) {
+    return (long long)p.pages.kv_heads * p.tiles * p.splits;
 }
 
 template <typename T, int D>
-static void go(const AttendParams& own, const Plan& plan, hipStream_t stream) {
-    constexpr bool tiled = sizeof(T) == 2 && D <= 256;
-    const bool tile = tiled && plan.rows > kRows, prefix_tile = tiled && plan.prefix_rows > kRows;
+static void go(const Attention& a, const Plan& plan, void* scratch, hipStream_t stream) {
+    typedef Forms<T, D> F;
+    AttendParams own{};
+    own.pages = a.pages;
+    own.batch = a.batch;
+    own.prefix_pages = a.prefix_pages;
+    own.prefix_len = a.prefix_len;
+    own.heads = a.heads;
+    own.group = FastDiv::of((unsigned)a.heads / a.pages.kv_heads);
+    own.q = a.q;
+    own.out = a.out;
+    own.qs = a.qs;
+    own.os = a.os;
+    // A scale of zero makes all scores equal; so does one that is next to it, and a
+    // masked score's -infinity stays one.
+    own.c2 = std::max(std::fabs(a.scale) * kLog2e, 1e-37f);
+    own.lag = std::min(kLag / own.c2, 1e30f);
+    own.sign = a.scale >= 0 ? 0 : a.dtype == XATTN_F32 ? 0x80000000u : 0x80008000u;
+    own.causal = a.causal;
+    own.tiles = plan.tiles;
+    own.single = plan.single;
+    own.splits = plan.own.splits;
+    own.chunk = plan.own.chunk;
+    own.slot = plan.prefix_parts(a.prefix_len);
+    own.slots = plan.slots();
+    if (const size_t n = parts(a, plan)) {
+        own.po = (float*)scratch;
+        own.ml = (float2*)(own.po + n * D);
+    }
+    AttendParams p = own;
+    p.single = 0;
+    p.tiles = plan.prefix_tiles;
+    p.splits = plan.prefix.splits;
+    p.chunk = plan.prefix.chunk;
+    p.slot = 0;
+    const long long units = (long long)own.batch.tokens * own.heads * (D > 256 ? D / 256 : 1);
+    const bool together = units < 8 * device_cu_count();
+    const unsigned merge = (unsigned)(together ? units : (units + kWaves - 1) / kWaves);
+    if (!grid_fits("cache attention", blocks(p) + blocks(own)) ||
+        !grid_fits("cache attention", merge))
+        return;
     if (plan.prefix.splits > 0) {
-        AttendParams p = own;
-        p.single = 0;
-        p.tiles = plan.prefix_tiles;
-        p.splits = plan.prefix.splits;
-        p.chunk = plan.prefix.chunk;
-        p.slot = 0;
-        const unsigned first = blocks(p), all = first + blocks(own);
-        if constexpr (tiled) {
-            if (tile)
-                cache_prefix_kernel<T, D, 2><<<all, 256, 0, stream>>>(p, own, first);
-            else if (prefix_tile)
-                cache_prefix_kernel<T, D, 1><<<all, 256, 0, stream>>>(p, own, first);
+        const unsigned first = (unsigned)blocks(p), all = first + (unsigned)blocks(own);
+        // a sequence has no more rows than the batch
+        if constexpr (F::kMany) {
+            if (plan.many)
+                cache_prefix_kernel<T, D, true, true><<<all, 256, 0, stream>>>(p, own, first);
+            else if (plan.prefix_many)
+                cache_prefix_kernel<T, D, true, false><<<all, 256, 0, stream>>>(p, own, first);
         }
-        if (!prefix_tile) cache_prefix_kernel<T, D, 0><<<all, 256, 0, stream>>>(p, own, first);
-    } else if (tile) {
-        if constexpr (tiled) cache_tile_kernel<T, D><<<blocks(own), 256, 0, stream>>>(own);
+        if (!plan.prefix_many)
+            cache_prefix_kernel<T, D, false, false><<<all, 256, 0, stream>>>(p, own, first);
+    } else if (!plan.many) {
+        cache_attend_kernel<T, D, false><<<(unsigned)blocks(own), 256, 0, stream>>>(own);
     } else {
-        cache_attend_kernel<T, D><<<blocks(own), 256, 0, stream>>>(own);
+        if constexpr (F::kMany)
+            cache_attend_kernel<T, D, true><<<(unsigned)blocks(own), 256, 0, stream>>>(own);
     }
-    if (own.po) {
-        const long long units = (long long)own.batch.tokens * own.heads * (D > 256 ? D / 256 : 1);
-        const bool together = units < 8 * device_cu_count();
-        cache_merge_kernel<T, D>
-            <<<(unsigned)(together ? units : (units + kWaves - 1) / kWaves), 256, 0, stream>>>(
-                own, own.slot, together);
-    }
+    if (own.po)
+        cache_merge_kernel<T, D><<<merge, 256, 0, stream>>>(own, own.slot, together);
 }
 
-template <typename T>
-static void by_dim(AttendParams& p, const Plan& plan, hipStream_t stream) {
-    if (p.pages.dim == 64) go<T, 64>(p, plan, stream);
-    if (p.pages.dim == 128) go<T, 128>(p, plan, stream);
-    if (p.pages.dim == 256) go<T, 256>(p, plan, stream);
-    if (p.pages.dim == kDim) go<T, kDim>(p, plan, stream);
+// f(T{}, dim as a constant) for the call's type and dim.
+template <typename F>
+static void dispatch(const Attention& a, F f) {
+    const auto by_dim = [&](auto type) {
+        if (a.pages.dim == 64) f(type, std::integral_constant<int, 64>{});
+        if (a.pages.dim == 128) f(type, std::integral_constant<int, 128>{});
+        if (a.pages.dim == 256) f(type, std::integral_constant<int, 256>{});
+        if (a.pages.dim == kDim) f(type, std::integral_constant<int, kDim>{});
+    };
+    if (a.dtype == XATTN_F32) by_dim(float{});
+    if (a.dtype == XATTN_F16) by_dim(_Float16{});
+    if (a.dtype == XATTN_BF16) by_dim(__bf16{});
+}
+
+size_t attention_scratch(const Attention& a) {
+    size_t n = 0;
+    dispatch(a, [&](auto type, auto dim) {
+        n = parts(a, plan<decltype(type), dim()>(a)) * (dim() * sizeof(float) + sizeof(float2));
+    });
+    return n;
 }
 
 bool launch_attention(const Attention& a, void* scratch, hipStream_t stream) {
-    const Plan pl = plan(a);
-    AttendParams p{};
-    p.pages = a.pages;
-    p.batch = a.batch;
-    p.prefix_pages = a.prefix_pages;
-    p.prefix_len = a.prefix_len;
-    p.heads = a.heads;
-    p.group = FastDiv::of((unsigned)a.heads / a.pages.kv_heads);
-    p.q = a.q;
-    p.out = a.out;
-    p.qs = a.qs;
-    p.os = a.os;
-    // A scale of zero makes all scores equal; so does one that is next to it, and a
-    // masked score's -infinity stays one.
-    p.c2 = std::max(std::fabs(a.scale) * kLog2e, 1e-37f);
-    p.lag = std::min(kLag / p.c2, 1e30f);
-    p.sign = a.scale >= 0 ? 0 : a.dtype == XATTN_F32 ? 0x80000000u : 0x80008000u;
-    p.causal = a.causal;
-    p.tiles = pl.tiles;
-    p.single = pl.single;
-    p.splits = pl.own.splits;
-    p.chunk = pl.own.chunk;
-    p.slot = pl.prefix_parts(a.prefix_len);
-    p.slots = pl.slots();
-    if (const size_t n = parts(a, pl)) {
-        p.po = (float*)scratch;
-        p.ml = (float2*)(p.po + n * a.pages.dim);
-    }
-    if (a.dtype == XATTN_F32) by_dim<float>(p, pl, stream);
-    if (a.dtype == XATTN_F16) by_dim<_Float16>(p, pl, stream);
-    if (a.dtype == XATTN_BF16) by_dim<__bf16>(p, pl, stream);
-    return check_launch("cache_attend_kernel");
+    dispatch(a, [&](auto type, auto dim) {
+        typedef decltype(type) T;
+        go<T, dim()>(a, plan<T, dim()>(a), scratch, stream);
+    });
+    return check_launch("cache attention");
 }
 
 }  // namespace cache

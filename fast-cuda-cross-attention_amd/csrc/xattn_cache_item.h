@@ -8,7 +8,7 @@
 namespace xattn {
 namespace cache {
 
-constexpr int kRows = 16;  // rows of a work item of attend_item and ring_item
+constexpr int kRows = 16;  // rows of a block: a matrix instruction's
 constexpr int kWaves = 4;
 
 struct AttendParams {
@@ -36,6 +36,8 @@ typedef unsigned int u4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
+typedef __attribute__((address_space(3))) u4 lds_u4;
+typedef __attribute__((address_space(3))) char lds_char;
 
 template <typename T> struct Vec8;
 template <> struct Vec8<_Float16> { typedef h8 type; };
@@ -109,6 +111,13 @@ __device__ inline f4 odd_values(const char* v) {
         y[e] = __builtin_isfinite(f) ? 0.0f : f;
     }
     return y;
+}
+
+// The weights of a tile's 32 keys as a matrix operand.
+template <typename T>
+__device__ inline u4 pack8(f4 lo, f4 hi) {
+    return u4{pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]), pack2<T>(hi[0], hi[1]),
+              pack2<T>(hi[2], hi[3])};
 }
 
 // A sequence as an item sees it.
@@ -229,7 +238,8 @@ __device__ inline bool find_item(const AttendParams& p, unsigned block, Item* it
         else if (!find_tile<ROWS>(p.batch, (int)p.group.d, (int)tile, &b, &local))
             return false;
         it->s = sequence(p.batch, b);
-        it->table = p.batch.page_table + (long long)b * p.batch.width;
+        it->table = p.batch.page_table +
+                    (long long)__builtin_amdgcn_readfirstlane(b) * p.batch.width;
     }
     it->causal = !PREFIX && p.causal;
     // The same in every lane, which the compiler cannot see.
@@ -238,7 +248,6 @@ __device__ inline bool find_item(const AttendParams& p, unsigned block, Item* it
     it->s.last = __builtin_amdgcn_readfirstlane(it->s.last);
     it->s.len = __builtin_amdgcn_readfirstlane(it->s.len);
     it->s.bad = __builtin_amdgcn_readfirstlane(it->s.bad);
-    it->table = uniform_ptr(it->table);
     local = __builtin_amdgcn_readfirstlane(local);
     const long long all = (long long)(it->s.end - it->s.first) * p.group.d;
     const long long row0 = (long long)local * ROWS;
@@ -274,47 +283,71 @@ __device__ inline void store(const AttendParams& p, const Item& it, int row, int
     }
 }
 
-// One tile of the running softmax of lane j's row: the scores of its keys, 4 g + i
-// of each sixteen, become weights relative to the row's maximum, which is raised
-// first; keys from `seen` on (key: that of sc[0][0]) weigh nothing.  *l is this
-// lane's share of the sum.  Returns the factor that the output takes.
-template <int H>
-__device__ inline float weights(const AttendParams& p, f4 (&sc)[H], bool partial, int key,
-                                int seen, float* m, float* l) {
-    if (partial)
+// One tile of the running softmax of RB rows of lane j: the scores of their keys,
+// 4 g + i of each sixteen, become weights relative to a maximum; keys from `seen` on
+// (key: that of sc[b][0][0]) weigh nothing.  The maximum m is raised only when a
+// score exceeds it by kLag (in exponents of 2), for all rows of the wavefront
+// together, so that the output is rarely rescaled: weights stay below 2^kLag, far
+// from the range of any type.  l is this lane's share of the sum.  True where
+// the output has to be multiplied by `keep`.
+constexpr float kLag = 8.0f;
+
+template <int RB, int H>
+__device__ inline bool weights(const AttendParams& p, f4 (&sc)[RB][H], bool partial, int key,
+                               const int (&seen)[RB], float (&m)[RB], float (&l)[RB],
+                               float (&keep)[RB]) {
+    if (partial) {
+        asm volatile("" : "+v"(key));  // keeps the comparisons in this branch
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (key + 16 * h + i >= seen[b]) sc[b][h][i] = -INFINITY;
+    }
+    float top[RB];
+    bool past = false;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        top[b] = -INFINITY;
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (key + 16 * h + i >= seen) sc[h][i] = -INFINITY;
-    float top = -INFINITY;
+            for (int i = 0; i < 4; ++i) top[b] = fmaxf(top[b], sc[b][h][i]);
+        top[b] = wave_max16_groups(top[b]);
+        past |= top[b] > m[b] + p.lag;
+    }
+    const bool raise = __ballot(past) != 0;
 #pragma unroll
-    for (int h = 0; h < H; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[h][i]);
-    top = fmaxf(*m, wave_max16_groups(top));
-    // exponents are taken from 0 while a row has seen nothing
-    const float ref = top == -INFINITY ? 0.0f : top * p.c2;
-    const float keep = top == *m ? 1.0f : fast_exp2(*m * p.c2 - ref);
-    *m = top;
-    float sum = *l * keep;
-#pragma unroll
-    for (int h = 0; h < H; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sc[h][i] = fast_exp2(__builtin_fmaf(sc[h][i], p.c2, -ref));
-            sum += sc[h][i];
+    for (int b = 0; b < RB; ++b) {
+        keep[b] = 1.0f;
+        if (raise) {
+            const float to = fmaxf(m[b], top[b]);
+            if (to != m[b]) keep[b] = fast_exp2((m[b] - to) * p.c2);
+            m[b] = to;
         }
-    *l = sum;
-    return keep;
+        // exponents are taken from 0 while a row has seen nothing
+        const float ref = m[b] == -INFINITY ? 0.0f : m[b] * p.c2;
+        float sum = l[b] * keep[b];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sc[b][h][i] = fast_exp2(__builtin_fmaf(sc[b][h][i], p.c2, -ref));
+                sum += sc[b][h][i];
+            }
+        l[b] = sum;
+    }
+    return raise;
 }
 
 // Joins the four wavefronts' results of the same rows over keys of their own: their
 // maxima and sums in `stats`, their output rows, row_floats apart, in every
 // wave_bytes of LDS.
-template <typename T, int D, bool PREFIX>
+template <typename T, int D, bool PREFIX, int ROWS>
 __device__ inline void join_and_store(const AttendParams& p, const Item& it,
-                                      const float2 (*stats)[kRows], const char* lds,
+                                      const float2 (*stats)[ROWS], const char* lds,
                                       int wave_bytes, int row_floats) {
     for (int i = threadIdx.x; i < it.rows * (D / 4); i += 256) {
         const int row = i / (D / 4), col = i % (D / 4) * 4;

@@ -1,28 +1,24 @@
-// Cache attention in 32 bits, and in 16 bits at dim 768 (ring_item): sixteen rows.
+// Cache attention in 16 bits at dim 768 (ring_item): RB blocks of sixteen rows, one or
+// two.
 //
-// The scores and weights lie in the lanes as in xattn_cache_few.h (16x16x4 MFMAs in
-// 32 bits: tiles of 16 keys, a weight's register is its operand's).  Up to dim 256
-// every wavefront has tiles of its own; at 768 the four share theirs and own 192
-// columns each, of Q, K, V and the output, and sum their shares of the scores
-// through LDS.
+// Operands, scores and weights as in xattn_cache_few.h.  The four wavefronts share
+// tiles of 32 keys and own 192 columns each, of Q, K, V and the output; their shares
+// of the scores are summed through LDS, one barrier a tile.
 //
-// K arrives by DMA in a slice of LDS of the wavefront's own.  Straight into the
+// K arrives by DMA in a slice of LDS of the wavefront's own: straight into the
 // operand's layout, whose neighbouring lanes are different rows, a KiB would hold
-// the CU's path to memory for 64 cycles instead of 16, which bounded this form at
-// 3.7 us a tile of 768 columns where the matrix instructions take 1.3.  Its pieces
-// are swizzled so that neighbouring rows use distinct banks.  V comes in whole rows
-// into registers: in 32 bits a lane's 16 bytes are one element each of four matrix
-// operands, whose columns are dealt accordingly (column 64 (b / 4) + 4 r + b % 4 is
-// row r of block b); in 16 bits they pass through LDS to be read transposed.
+// the CU's path to memory for 64 cycles instead of 16.  Its pieces are swizzled so
+// that neighbouring rows use distinct banks.  V comes in whole rows into registers
+// and passes through LDS to be read transposed.
 //
 // A tile's scores come before the product of the tile before it with V, under which
-// the shares of the scores are exchanged; its softmax comes last.  What the next
-// steps need is asked for piece by piece between the matrix instructions (in one
-// run it would hold the wavefront until the path to memory has taken it, 968 cycles
-// for V at 768 columns in 32 bits): in 32 bits the next K under the scores, into the
-// other of two slots, and this tile's V under the product, register by register as
-// the old ones have been used; in 16 bits, whose LDS has room for one K only, the
-// next K under the product and V behind it.
+// the next K is asked for, piece by piece, and the shares of the scores are
+// exchanged; then V of this tile is asked for, and its softmax done.  So everything
+// that arrives has a product's time or more to do so, and LDS need hold one K.
+//
+// Bound by that path: a tile of K and V is 96 KiB, 1,536 cycles, against 384 RB of
+// matrix instructions.  32 sequences of 4,000 keys, one token each, are read at
+// 4.9 TB/s; 64 rows over 50,176 keys take 69 us with two blocks and 79 with one.
 #pragma once
 
 #include "xattn_cache_item.h"
@@ -30,72 +26,58 @@
 namespace xattn {
 namespace cache {
 
-template <typename T, int D>
+template <int RB>
 struct RingShape {
-    static constexpr bool kWide = sizeof(T) == 4;
-    static constexpr int kCols = D > 256 ? kWaves : 1;  // wavefronts that share a tile
-    static constexpr int kDW = D / kCols;               // columns of a wavefront
-    static constexpr int kKeys = kWide ? 16 : 32;       // keys of a tile
+    static constexpr int kDW = kDim / kWaves;           // columns of a wavefront
+    static constexpr int kKeys = 32;                    // keys of a tile
     static constexpr int kRegs = kDW / 16;              // KiB of a wavefront's K, or V, in a tile
     static constexpr int kBlocks = kDW / 16;            // 16-column blocks of the output
-    static constexpr int kRow = kDW * (int)sizeof(T);   // bytes of a row's columns
+    static constexpr int kRow = kDW * 2;                // bytes of a row's columns
     static constexpr int kPieces = kRow / 16;
     // A KiB holds 64 pieces of consecutive rows; kPeriod KiB hold kStep whole rows.
-    static constexpr int kPeriod =
-        64 % kPieces == 0 ? 1 : kPieces % 16 == 0 ? kPieces / 16 : kPieces / 8;
-    static constexpr int kStep = 64 * kPeriod / kPieces;
+    static constexpr int kPeriod = 3, kStep = 8;
+    static_assert(kPeriod * 64 == kStep * kPieces, "whole rows");
     static constexpr int kKTile = kRegs * 1024;
-    static constexpr int kSlots = kWide ? 2 : 1;        // K tiles of a wavefront in LDS
     static constexpr int kVRow = kRow + 32;             // in LDS; 32 bytes of padding deal four
                                                         // rows to distinct banks
-    static constexpr int kVTile = kWide ? 0 : kKeys * kVRow;
-    static constexpr int kORow = kDW + 4;               // floats of an output row in LDS
-    static constexpr int kOut = kCols > 1 ? 0 : kRows * kORow * 4;
-    static constexpr int kTiles = kSlots * kKTile + kVTile;
-    static constexpr int kWaveLds = kTiles > kOut ? kTiles : kOut;
-    static constexpr int kShare = kKeys * kRows * 4;    // bytes of a wavefront's share of scores
-    static constexpr int kShares = kCols > 1 ? 2 * kWaves * kShare : 0;
-    static constexpr int kStats = kWaves * kRows * 8;   // maxima and sums
-    static constexpr int kLds = kWaves * kWaveLds + kShares + kStats;
-    // What a row's piece numbers in LDS are xored with: eight rows put a column's
-    // 32 bytes into eight different eighths of the banks.
-    static constexpr __device__ int swizzle(int row) {
-        return kRow % 256 == 0 ? row % 8 * 2 : row / 2 % 4 * 2;
-    }
+    static constexpr int kWaveLds = kKTile + kKeys * kVRow;
+    static constexpr int kShare = RB * kKeys * kRows * 4;  // bytes of a wavefront's share of scores
+    static constexpr int kLds = kWaves * kWaveLds + 2 * kWaves * kShare;
 };
 
-template <typename T, int D, bool PREFIX>
+template <typename T, int RB, bool PREFIX>
 __device__ __forceinline__ void ring_item(const AttendParams& p, unsigned block, char* lds) {
-    typedef RingShape<T, D> S;
-    constexpr int KT = S::kKeys, KB = KT / 16, NR = S::kRegs, NB = S::kBlocks;
-    constexpr bool WIDE = S::kWide, SHARED = S::kCols > 1;
-    constexpr int PERIOD = S::kPeriod, STEP = S::kStep, SIZE = (int)sizeof(T), ROW = D * SIZE;
-    float2(*const stats)[kRows] = (float2(*)[kRows])(lds + S::kLds - S::kStats);
+    typedef RingShape<RB> S;
+    constexpr int KT = S::kKeys, KB = KT / 16, NR = S::kRegs, NB = S::kBlocks, NQ = NR / 2;
+    constexpr int PERIOD = S::kPeriod, STEP = S::kStep, ROW = kDim * 2;
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int j = lane % 16, g = lane / 16;
 
     Item it;
-    if (!find_item<kRows, PREFIX>(p, block, &it)) return;
+    if (!find_item<RB * kRows, PREFIX>(p, block, &it)) return;
     const Sequence& s = it.s;
     const int least = it.least, k0 = it.k0, k1 = it.k1;
-    const Row mine = it.row(p, min(j, it.rows - 1));
-    const int seen = min(s.seen(mine.token, it.causal), k1);
 
-    // Q: register r holds elements 16 r + 4 g on (32 bits), 32 r + 8 g on (16 bits).
-    constexpr int NQ = WIDE ? NR : NR / 2;
-    const int col0 = SHARED ? wave * S::kDW : 0;
-    u4 qr[NQ];
-    {
-        const char* q = (const char*)((const T*)p.q + mine.token * p.qs +
-                                      (long long)mine.head * D + col0) + 16 * g;
+    // Q: register r of lane (j, g) holds elements 32 r + 8 g .. + 7 of row j.
+    const int col0 = wave * S::kDW;
+    int seen[RB];
+    u4 qr[RB][NQ];
+    f4 o[RB][NB];
+    float m[RB], l[RB];
 #pragma unroll
-        for (int r = 0; r < NQ; ++r) qr[r] = *(const u4*)(q + 64 * r) ^ p.sign;
+    for (int b = 0; b < RB; ++b) {
+        const Row mine = it.row(p, min(kRows * b + j, it.rows - 1));
+        seen[b] = min(s.seen(mine.token, it.causal), k1);
+        const T* q =
+            (const T*)p.q + mine.token * p.qs + (long long)mine.head * kDim + col0 + 8 * g;
+#pragma unroll
+        for (int r = 0; r < NQ; ++r) qr[b][r] = *(const u4*)(q + 32 * r) ^ p.sign;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) o[b][i] = f4{0, 0, 0, 0};
+        m[b] = -INFINITY;
+        l[b] = 0.0f;
     }
-    f4 o[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) o[b] = f4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;
     bool bad = false, odd = false;
 
     // Where a tile's rows are.  Sixteen rows lie on one page where sixteen divides
@@ -112,227 +94,164 @@ __device__ __forceinline__ void ring_item(const AttendParams& p, unsigned block,
         return ((ok ? (unsigned)page : 0u) * p.pages.kv_heads + it.kv_head) * size +
                (key - p.pages.page_size.div(key) * size);
     };
-    const auto half = [&](const char* pool, int ids, int k, int h) {  // rows 16 h on
-        const unsigned row = row_at(__builtin_amdgcn_readlane(ids, 16 * h), k + 16 * h);
-        return pool + (size_t)row * ROW + col0 * SIZE;
+    const auto halves = [&](int ids, int k, size_t (&from)[KB]) {  // byte offsets, scalars
+#pragma unroll
+        for (int h = 0; h < KB; ++h) {
+            const unsigned row = row_at(__builtin_amdgcn_readlane(ids, 16 * h), k + 16 * h);
+            from[h] = (size_t)row * ROW + col0 * 2;
+        }
     };
     const auto one = [&](const char* pool, int ids, int k, int r) {  // row r
         const unsigned row = row_at(__shfl(ids, r), (unsigned)min(k + r, k1 - 1));
-        return pool + (size_t)row * ROW + col0 * SIZE;
+        return pool + (size_t)row * ROW + col0 * 2;
+    };
+    // (The lane read through an empty asm: what the rare paths derive from it is
+    // otherwise kept in registers across the loop.)
+    const auto hidden_lane = [&]() {
+        int i = lane;
+        asm volatile("" : "+v"(i));
+        return i;
     };
 
     // K by DMA: KiB c of a tile.
     char* const kt = lds + wave * S::kWaveLds;
     const unsigned kt_at = __builtin_amdgcn_readfirstlane(lds_u32(kt));
-    int k_row[PERIOD], k_piece[PERIOD];
+    const auto swizzle = [](int row) { return row / 2 % 4 * 2; };
+    int row_of[PERIOD], piece_of[PERIOD];
 #pragma unroll
     for (int i = 0; i < PERIOD; ++i) {
-        k_row[i] = (i * 64 + lane) / S::kPieces;
-        k_piece[i] = (i * 64 + lane) % S::kPieces;
+        row_of[i] = (i * 64 + lane) / S::kPieces;
+        piece_of[i] = (i * 64 + lane) % S::kPieces;
     }
-    const auto k_from = [&](int c) {  // lane's piece of its row's columns, in bytes
-        const int row = STEP * (c / PERIOD) + k_row[c % PERIOD];
-        return 16 * (k_piece[c % PERIOD] ^ S::swizzle(row));
+    const DmaSrc pool = dma_base(p.pages.k);
+    const auto k_whole = [&](const size_t (&from)[KB], int c) {
+        const int row = STEP * (c / PERIOD), i = c % PERIOD;
+        dma16_m0<0>(pool + (from[row / 16] + (size_t)(row % 16 * ROW)),
+                    (unsigned)(row_of[i] * ROW + 16 * (piece_of[i] ^ swizzle(row + row_of[i]))),
+                    kt_at + 1024 * c);
     };
-    const auto dma_whole = [&](const DmaSrc (&from)[KB], int slot, int c) {
-        const int row = STEP * (c / PERIOD);
-        dma16_m0<0>(from[row / 16] + (size_t)(row % 16 * ROW),
-                    (unsigned)(k_row[c % PERIOD] * ROW + k_from(c)),
-                    kt_at + slot * S::kKTile + 1024 * c);
-    };
-    DmaSrc pool;
-    {
-        DmaSrc same;
-        dma_base2(p.pages.k, p.pages.k, pool, same);
-    }
-    const auto k_whole = [&](int ids, int k, DmaSrc (&from)[KB]) {
+    const auto k_any = [&](int ids, int k) {
+        const int me = hidden_lane();
 #pragma unroll
-        for (int h = 0; h < KB; ++h)
-            from[h] = pool + (size_t)(half(p.pages.k, ids, k, h) - p.pages.k);
-    };
-    const auto dma_any = [&](int ids, int k, int slot) {
-#pragma unroll
-        for (int c = 0; c < NR; ++c)
-            dma16_lanes(one(p.pages.k, ids, k, STEP * (c / PERIOD) + k_row[c % PERIOD]) + k_from(c),
-                        kt_at + slot * S::kKTile + 1024 * c);
-    };
-
-    // V in registers.  32 bits: register r is columns 64 (r / 4) + 4 j on of row 4 g +
-    // r % 4.  16 bits: KiB r in row order.
-    u4 vr[NR];
-    const auto v_whole = [&](int ids, int k, const char* (&from)[KB]) {
-#pragma unroll
-        for (int h = 0; h < KB; ++h) from[h] = half(p.pages.v, ids, k, h);
-    };
-    const auto load_whole = [&](const char* const (&from)[KB], int r) {
-        if constexpr (WIDE) {
-            const unsigned at = 4 * g * ROW + 16 * j;
-            vr[r] = *(const u4*)(from[0] + (r % 4 * ROW + 256 * (r / 4)) + at);
-        } else {
-            const int row = STEP * (r / PERIOD);
-            const unsigned at = k_row[r % PERIOD] * ROW + 16 * k_piece[r % PERIOD];
-            vr[r] = *(const u4*)(from[row / 16] + row % 16 * ROW + at);
+        for (int c = 0; c < NR; ++c) {
+            const int i = c % PERIOD * 64 + me, row = STEP * (c / PERIOD) + i / S::kPieces;
+            dma16_lanes(one(p.pages.k, ids, k, row) + 16 * (i % S::kPieces ^ swizzle(row)),
+                        kt_at + 1024 * c);
         }
     };
-    const auto load_any = [&](int ids, int k) {
+
+    // V in registers: KiB r in row order.
+    u4 vr[NR];
+    const auto v_whole = [&](const size_t (&from)[KB]) {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            if constexpr (WIDE)
-                vr[r] = *(const u4*)(one(p.pages.v, ids, k, 4 * g + r % 4) + 256 * (r / 4) + 16 * j);
-            else
-                vr[r] = *(const u4*)(one(p.pages.v, ids, k,
-                                         STEP * (r / PERIOD) + k_row[r % PERIOD]) +
-                                     16 * k_piece[r % PERIOD]);
+            const int row = STEP * (r / PERIOD), i = r % PERIOD;
+            const unsigned at = row_of[i] * ROW + 16 * piece_of[i];
+            vr[r] = *(const u4*)(p.pages.v + (from[row / 16] + row % 16 * ROW) + at);
+        }
+    };
+    const auto v_any = [&](int ids, int k) {
+        const int me = hidden_lane();
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int i = r % PERIOD * 64 + me;
+            vr[r] = *(const u4*)(one(p.pages.v, ids, k, STEP * (r / PERIOD) + i / S::kPieces) +
+                                 i % S::kPieces * 16);
         }
     };
 
-    // The product of the weights `w` with the V in registers.  Between its steps comes
-    // also(r); in 32 bits V's register r is free by then.
-    char* const vt = kt + S::kSlots * S::kKTile;
-    f4 w[KB];
+    // The product of the weights w with the V in registers; also(i) amid its steps.
+    char* const vt = kt + S::kKTile;
+    u4 w[RB];
     const auto product = [&](auto also) {
-        if constexpr (WIDE) {
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
+        for (int r = 0; r < NR; ++r)
+            *(u4*)(vt + (STEP * (r / PERIOD) + row_of[r % PERIOD]) * S::kVRow +
+                   16 * piece_of[r % PERIOD]) = vr[r];
+        const char* from = vt + (4 * g + j / 4) * S::kVRow + j % 4 * 8;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    o[r / 4 * 4 + e] =
-                        mfma4(__uint_as_float(vr[r][e]), w[0][r % 4], o[r / 4 * 4 + e]);
-                also(r);
-            }
-        } else {
+        for (int i = 0; i < NB; ++i) {
+            also(i);
+            const u4 v = transposed(from + 32 * i, from + 32 * i + 16 * S::kVRow);
 #pragma unroll
-            for (int r = 0; r < NR; ++r)
-                *(u4*)(vt + (STEP * (r / PERIOD) + k_row[r % PERIOD]) * S::kVRow +
-                       16 * k_piece[r % PERIOD]) = vr[r];
-            const u4 x = {pack2<T>(w[0][0], w[0][1]), pack2<T>(w[0][2], w[0][3]),
-                          pack2<T>(w[KB - 1][0], w[KB - 1][1]), pack2<T>(w[KB - 1][2], w[KB - 1][3])};
-            const char* from = vt + (4 * g + j / 4) * S::kVRow + j % 4 * 8;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                also(b);
-                o[b] = mfma32<T>(transposed(from + 32 * b, from + 32 * b + 16 * S::kVRow), x, o[b]);
-            }
+            for (int b = 0; b < RB; ++b) o[b][i] = mfma32<T>(v, w[b], o[b][i]);
         }
     };
+    const auto meet = [&](int i) {
+        if (i == NB / 2) lds_barrier();
+    };
 
-    const int step = SHARED ? KT : kWaves * KT;
-    int k = k0 + (SHARED ? 0 : wave * KT);
-    if (k < k1) {
-        int ids = find(k), ids1 = find(k + step);
-        dma_any(ids, k, 0);
+    if (k0 < k1) {
+        // Pages of this tile (`ids`) and the next (`ids1`), and where whole tiles of the
+        // two begin: K of the next tile and, a step later, its V lie alike.
+        int ids = find(k0), ids1 = find(k0 + KT);
+        size_t at[KB] = {}, at1[KB] = {};
+        k_any(ids, k0);
         wait_vmcnt<0>();
         bool first = true, partial = false;
-        for (int turn = 0; k < k1; k += step, turn ^= 1) {
-            const bool more = k + step < k1, whole = runs && k + KT <= k1;
-            const bool whole1 = more && runs && k + step + KT <= k1;
-            const int ids2 = find(k + 2 * step);
-            f4 sc[KB];
-            if constexpr (WIDE) {
-                // in four sums, as a product takes longer to come out than to start
-                const char* const from = kt + turn * S::kKTile + j * S::kRow;
-                const auto scores = [&](auto also) {
-                    f4 part[4];
+        for (int k = k0, turn = 0; k < k1; k += KT, turn ^= 1) {
+            const bool more = k + KT < k1, whole = runs && k + KT <= k1;
+            const bool whole1 = more && runs && k + 2 * KT <= k1;
+            if (whole1) halves(ids1, k + KT, at1);
+            f4 sc[RB][KB];
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        const u4 a = *(const u4*)(from + 16 * (4 * r + g ^ S::swizzle(j)));
-                        also(r);
+            for (int r = 0; r < NQ; ++r)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            part[e] = mfma4(__uint_as_float(a[e]), __uint_as_float(qr[r][e]),
-                                            r ? part[e] : f4{0, 0, 0, 0});
-                    }
-                    sc[0] = (part[0] + part[1]) + (part[2] + part[3]);
-                };
-                if (whole1) {
-                    DmaSrc next[KB];
-                    k_whole(ids1, k + step, next);
-                    scores([&](int r) { dma_whole(next, turn ^ 1, r); });
-                } else {
-                    if (more) dma_any(ids1, k + step, turn ^ 1);
-                    scores([](int) {});
+                for (int h = 0; h < KB; ++h) {
+                    const u4 a = *(const u4*)(kt + (16 * h + j) * S::kRow +
+                                              16 * (4 * r + g ^ swizzle(j)));
+#pragma unroll
+                    for (int b = 0; b < RB; ++b)
+                        sc[b][h] = mfma32<T>(a, qr[b][r], r ? sc[b][h] : f4{0, 0, 0, 0});
                 }
-            } else {
+            char* const share =
+                lds + kWaves * S::kWaveLds + turn * kWaves * S::kShare + lane * 16;
 #pragma unroll
-                for (int r = 0; r < NQ; ++r)
-#pragma unroll
-                    for (int h = 0; h < KB; ++h) {
-                        const u4 a = *(const u4*)(kt + (16 * h + j) * S::kRow +
-                                                  16 * (4 * r + g ^ S::swizzle(j)));
-                        sc[h] = mfma32<T>(a, qr[r], r ? sc[h] : f4{0, 0, 0, 0});
-                    }
-            }
-            char* const share = lds + kWaves * S::kWaveLds + turn * kWaves * S::kShare;
-            if constexpr (SHARED)
-#pragma unroll
-                for (int h = 0; h < KB; ++h)
-                    *(f4*)(share + wave * S::kShare + (h * kWave + lane) * 16) = sc[h];
-            // The product of the tile before.
+            for (int i = 0; i < RB * KB; ++i)
+                *(f4*)(share + wave * S::kShare + i * kWave * 16) = sc[i / KB][i % KB];
             if (!first && partial)
 #pragma unroll
                 for (int r = 0; r < NR; ++r) odd |= clear_not_finite<T>(vr[r]);
-            const auto meet = [&](int r) {
-                if constexpr (SHARED)
-                    if (r == NR / 2) lds_barrier();
-            };
-            if constexpr (WIDE) {
-                if (!first && whole) {
-                    const char* from[KB];
-                    v_whole(ids, k, from);
-                    product([&](int r) {
-                        load_whole(from, r);
-                        meet(r);
-                    });
-                } else {
-                    if (first)
-                        meet(NR / 2);
-                    else
-                        product(meet);
-                    load_any(ids, k);
-                }
+            if (more) wait_lds();  // this K has been read
+            if (!first && whole1) {
+                product([&](int i) {
+                    k_whole(at1, i);
+                    meet(i);
+                });
             } else {
-                if (more) wait_lds();  // this K has been read
-                if (!first && whole1) {
-                    DmaSrc next[KB];
-                    k_whole(ids1, k + step, next);
-                    product([&](int r) {
-                        dma_whole(next, 0, r);
-                        meet(r);
-                    });
-                } else {
-                    if (more) dma_any(ids1, k + step, 0);
-                    if (first)
-                        meet(NR / 2);
-                    else
-                        product(meet);
-                }
-                if (whole) {
-                    const char* from[KB];
-                    v_whole(ids, k, from);
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) load_whole(from, r);
-                } else {
-                    load_any(ids, k);
-                }
+                if (more) k_any(ids1, k + KT);
+                if (first)
+                    meet(NB / 2);
+                else
+                    product(meet);
             }
-            if constexpr (SHARED)
-#pragma unroll
-                for (int h = 0; h < KB; ++h) {
-                    sc[h] = *(f4*)(share + (h * kWave + lane) * 16);
-#pragma unroll
-                    for (int i = 1; i < kWaves; ++i)
-                        sc[h] += *(f4*)(share + i * S::kShare + (h * kWave + lane) * 16);
-                }
-            partial = k + KT > least;  // some row does not see all of the tile
-            const float keep = weights(p, sc, partial, k + 4 * g, seen, &m, &l);
-            if (__ballot(keep != 1.0f))
-#pragma unroll
-                for (int b = 0; b < NB; ++b) o[b] *= keep;
-#pragma unroll
-            for (int h = 0; h < KB; ++h) w[h] = sc[h];
-            first = false;
+            const int after = find(k + 2 * KT);
+            if (!first && whole)
+                v_whole(at);
+            else
+                v_any(ids, k);
             ids = ids1;
-            ids1 = ids2;
+            ids1 = after;
+#pragma unroll
+            for (int i = 0; i < RB * KB; ++i) {
+                f4 sum = *(f4*)(share + i * kWave * 16);
+#pragma unroll
+                for (int u = 1; u < kWaves; ++u)
+                    sum += *(f4*)(share + u * S::kShare + i * kWave * 16);
+                sc[i / KB][i % KB] = sum;
+            }
+            partial = k + KT > least;  // some row does not see all of the tile
+            float keep[RB];
+            if (weights(p, sc, partial, k + 4 * g, seen, m, l, keep))
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) o[b][i] *= keep[b];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) w[b] = pack8<T>(sc[b][0], sc[b][1]);
+            first = false;
+#pragma unroll
+            for (int h = 0; h < KB; ++h) at[h] = at1[h];
             // The next K has arrived: it was asked for before the NR loads of this V.
             if (more) wait_vmcnt<NR>();
         }
@@ -342,53 +261,25 @@ __device__ __forceinline__ void ring_item(const AttendParams& p, unsigned block,
         product([](int) {});
     }
     if (__ballot(odd))
-        for (int t = k0 + (SHARED ? 0 : wave * KT); t < k1; t += step)
-            for (int c = t; t + KT > least && c < min(t + KT, k1); ++c)
-                if (const char* v = it.row_of_v(p, c, ROW))
+        for (int c = max(k0, least / KT * KT); c < k1; ++c)
+            if (const char* v = it.row_of_v(p, c, ROW))
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        f4 x;
-                        if constexpr (WIDE) {
+                for (int i = 0; i < NB; ++i) {
+                    const f4 x = odd_values<T>(v + (col0 + 16 * i + 4 * g) * 2);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float f = *(const float*)(
-                                    v + (col0 + 64 * (b / 4) + 16 * g + 4 * i + b % 4) * 4);
-                                x[i] = __builtin_isfinite(f) ? 0.0f : f;
-                            }
-                        } else {
-                            x = odd_values<T>(v + (col0 + 16 * b + 4 * g) * 2);
-                        }
-                        if (c < seen) o[b] += x;
-                    }
-    l = wave_sum16_groups(l);
-    if (__ballot(bad)) l = NAN;
-
-    // In 32 bits four blocks hold four neighbouring columns each.
-    const auto quads = [&](auto put) {
+                    for (int b = 0; b < RB; ++b)
+                        if (c < seen[b]) o[b][i] += x;
+                }
+    const bool none = __ballot(bad) != 0;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if constexpr (WIDE) {
-                if (b % 4 == 0)
+    for (int b = 0; b < RB; ++b) {
+        const float sum = none ? NAN : wave_sum16_groups(l[b]);
+        const int row = kRows * b + j;
+        if (row < it.rows)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        put(16 * b + 16 * g + 4 * i,
-                            f4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]});
-            } else {
-                put(16 * b + 4 * g, o[b]);
-            }
-        }
-    };
-    if constexpr (SHARED) {
-        if (j < it.rows)
-            quads([&](int col, f4 x) {
-                store<T, D, PREFIX>(p, it, j, col0 + col, x, m * p.c2, l);
-            });
-    } else {
-        if (lane < kRows) stats[wave][lane] = {m * p.c2, l};
-        float* part = (float*)kt + j * S::kORow;
-        quads([&](int col, f4 x) { *(f4*)(part + col) = x; });
-        __syncthreads();
-        join_and_store<T, D, PREFIX>(p, it, stats, lds, S::kWaveLds, S::kORow);
+            for (int i = 0; i < NB; ++i)
+                store<T, kDim, PREFIX>(p, it, row, col0 + 16 * i + 4 * g, o[b][i], m[b] * p.c2,
+                                       sum);
     }
 }
 

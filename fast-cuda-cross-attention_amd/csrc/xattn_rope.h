@@ -241,7 +241,9 @@ static void go(RopeParams& p, hipStream_t stream) {
     p.units = FastDiv::of(H::units(p.dim, p.rope.rot));
     p.by_heads = FastDiv::of(p.heads);
     p.per = tokens_per_workgroup(p.tokens, (long long)p.heads * p.units.d, p.rope.rot / 2);
-    rope_kernel<T, V, IL><<<(p.tokens + p.per - 1) / p.per, kThreads, 0, stream>>>(p);
+    const long long blocks = ((long long)p.tokens + p.per - 1) / p.per;
+    if (grid_fits("rope_kernel", blocks))
+        rope_kernel<T, V, IL><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
 }
 
 template <typename T, int V, bool IL>
@@ -252,8 +254,9 @@ static void go(AppendParams& p, hipStream_t stream) {
     p.by_token = FastDiv::of((p.heads + p.pages.kv_heads) * p.units.d +
                              p.pages.kv_heads * p.copies.d);
     p.per = tokens_per_workgroup(p.batch.tokens, p.by_token.d, p.rope.rot / 2);
-    cache_append_kernel<T, V, IL>
-        <<<(p.batch.tokens + p.per - 1) / p.per, kThreads, 0, stream>>>(p);
+    const long long blocks = ((long long)p.batch.tokens + p.per - 1) / p.per;
+    if (grid_fits("cache_append_kernel", blocks))
+        cache_append_kernel<T, V, IL><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
 }
 
 template <typename T, typename P>

@@ -257,14 +257,15 @@ typedef struct xattn_batch {
     const int* kv_lens;    /* device, [batch] */
     const int* page_table; /* device, [batch][table_width] */
     int batch;
-    int table_width;
+    int table_width;       /* table_width * page_size <= 2^30 */
     int tokens;     /* rows of the token tensors, >= q_starts[batch] */
     int max_q_len;  /* at least the longest sequence's new tokens */
     int max_kv_len; /* about the longest kv_lens: the work is divided by it */
 } xattn_batch;
 
 /* Keys that every sequence of a batch sees before its own: positions 0 ..
- * len - 1 on pages[0 .. num_listed - 1], len <= num_listed * page_size. */
+ * len - 1 on pages[0 .. num_listed - 1], len <= num_listed * page_size and
+ * <= 2^30. */
 typedef struct xattn_prefix {
     const int* pages; /* device, [num_listed] */
     int num_listed;
@@ -330,8 +331,9 @@ size_t xattn_cache_attention_scratch(const xattn_kv_cache* cache, const xattn_ba
  * see do not count, whatever they hold (infinities and NaN included); a token
  * that sees none gets zeros.  dim 64, 128, 256 or 768.  out may not overlap q.
  * The tokens of a sequence come out as NaN if its length is negative or
- * beyond its row of page_table, or if a page that they see has a number
- * outside 0 .. num_pages - 1; those past max_q_len are left as they are.
+ * beyond its row of page_table, and those that see a page with a number
+ * outside 0 .. num_pages - 1 do (others of that sequence may).  Those of a
+ * sequence with more than max_q_len new ones are unspecified.
  * scratch: scratch_bytes >= xattn_cache_attention_scratch bytes, 16-byte
  * aligned, of this call alone until it has finished: calls (and replays of
  * graphs) that may overlap need scratch of their own.  Its contents need no
