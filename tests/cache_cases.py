@@ -33,6 +33,18 @@ class Batch:
         for b, n in enumerate(counts):
             self.page_table[b, :n], order = order[:n], order[n:]
 
+    def widen(self, keys):
+        """Rows of page_table for `keys` keys, and as many announced."""
+        more = -(-keys // self.page_size) - self.page_table.shape[1]
+        self.page_table = np.pad(self.page_table, ((0, 0), (0, max(more, 0))), constant_values=-7)
+        self.max_kv_len = lambda: keys
+
+    def max_q_len(self):
+        return max(self.q_lens, default=0)
+
+    def max_kv_len(self):
+        return int(max(self.kv_lens, default=0))
+
     @property
     def where(self):
         return self.q_starts, self.kv_lens, self.page_table
@@ -70,8 +82,7 @@ class OnDevice:
         self.batch = cw.BatchArgs(self.q_starts.ptr.value, self.kv_lens.ptr.value,
                                   self.table.ptr.value, len(batch.kv_lens),
                                   batch.page_table.shape[1], batch.tokens,
-                                  max(batch.q_lens, default=0),
-                                  int(max(batch.kv_lens, default=0)))
+                                  batch.max_q_len(), batch.max_kv_len())
         self.prefix = None
         if batch.prefix_len:
             self.listed = self.put(batch.prefix_pages)

@@ -236,3 +236,43 @@ def test_host_api_refusals(cw):
         cw.PagedCache(0, 16, 1, 64)
     with pytest.raises(ValueError):
         cw.PagedCache(1, 16, 1, 64, "fp8")
+
+
+# --------------------------------------------------------------------------
+# Sizes past a launch's grid, and positions past an int's sums
+# --------------------------------------------------------------------------
+
+WIDE = dict(dim=2048, rot=2048)
+
+
+def test_more_workgroups_than_a_grid_has(cw):
+    many = 1 << 26
+    got, msg = _rope(cw, tokens=many, heads=1, xs=2048, ys=2048, **WIDE)
+    assert got == UNSUPPORTED and "workgroups" in msg, (got, msg)
+    got, msg = _append(cw, tokens=many, kv_heads=1, heads=1, ks=2048, vs=2048, qs=2048, qos=2048,
+                       **WIDE)
+    assert got == UNSUPPORTED and "workgroups" in msg, (got, msg)
+    for with_prefix in (False, True):
+        got, msg = _attend(cw, with_prefix=with_prefix, tokens=many, batch=many, max_q_len=1,
+                           kv_heads=1, heads=1, qs=64, os=64)
+        assert got == UNSUPPORTED and "workgroups" in msg, (got, msg)
+
+
+def test_more_keys_than_positions_go_to(cw):
+    for call in (_append, _attend):
+        got, msg = call(cw, table_width=(1 << 26) + 1)
+        assert got == UNSUPPORTED and "2^30" in msg, (got, msg)
+    got, msg = _attend(cw, with_prefix=True, listed=1 << 27, len=(1 << 30) + 1)
+    assert got == UNSUPPORTED and "2^30" in msg, (got, msg)
+
+
+def test_work_is_not_divided_without_need(cw):
+    """Short sequences, and as many as the device has room for, need no scratch."""
+    def need(**kw):
+        cache, batch = _args(cw, **kw)
+        return cw.lib.xattn_cache_attention_scratch(ctypes.byref(cache), ctypes.byref(batch), None,
+                                                    4)
+    assert need(tokens=1, batch=1, max_q_len=1, max_kv_len=60) == 0
+    assert need(tokens=1, batch=1, max_q_len=1, max_kv_len=60000, table_width=10000) > 0
+    assert need(tokens=4096, batch=4096, max_q_len=1, max_kv_len=60000, table_width=10000) == 0
+    assert cw.HAS_CACHE
