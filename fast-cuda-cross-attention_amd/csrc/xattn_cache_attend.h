@@ -61,6 +61,8 @@ struct Forms {
     static constexpr int max_lds(bool a, bool b) { return lds(a) > lds(b) ? lds(a) : lds(b); }
     // Wavefronts that a SIMD has to hold: two of tile_item, in 256 registers each.
     static constexpr int waves(bool many) { return !kWide && !kRing && many ? 2 : 1; }
+    // Workgroups of tile_item that a CU holds.
+    static constexpr int kResident = D == 64 ? 3 : 2;
     template <bool MANY, bool PREFIX>
     static __device__ __forceinline__ void item(const AttendParams& p, unsigned block, char* lds) {
         if constexpr (kWide)
@@ -95,21 +97,40 @@ cache_prefix_kernel(AttendParams prefix, AttendParams own, unsigned prefix_block
 
 // --------------------------------------------------------------------------
 // cache_merge_kernel: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the
-// parts of a row.  A wavefront takes 256 columns of a row, or all of them, in
-// 64 / LANES groups of LANES lanes that take every so many-th part; with
-// `together` the four wavefronts of a workgroup share a row's parts (few rows of
-// many parts), otherwise each has a row of its own.
+// parts of a row.  LANES lanes take 256 columns of a row, or all of them.  Few
+// rows of many parts (TOGETHER): a workgroup a row, its groups of LANES lanes taking
+// every so many-th part.  Otherwise a group a row, those of a wavefront heads of
+// one token: what a row waits for are four reads one after another (its sequence,
+// length, maxima, parts), so many rows have to wait at once (20,860 rows of up to
+// four parts of 64: 13.0 us with a wavefront a row, 7.4 with a group).
 // --------------------------------------------------------------------------
-template <typename T, int D>
-__global__ __launch_bounds__(256) void cache_merge_kernel(AttendParams p, int prefix_parts,
-                                                          int together) {
-    constexpr int COLS = D > 256 ? 256 : D, LANES = COLS / 4, GROUPS = kWave / LANES;
+template <int D>
+struct MergeShape {
+    static constexpr int kCols = D > 256 ? 256 : D, kLanes = kCols / 4;
+    static constexpr int kGroups = kWave / kLanes;
+    // Wavefronts of a call, workgroups if TOGETHER.
+    static long long units(int tokens, int heads, bool together) {
+        const int per = together ? 1 : kGroups;
+        return (long long)tokens * (D / kCols) * ((heads + per - 1) / per);
+    }
+};
+
+template <typename T, int D, bool TOGETHER>
+__global__ __launch_bounds__(256) void cache_merge_kernel(AttendParams p, int prefix_parts) {
+    typedef MergeShape<D> S;
+    constexpr int COLS = S::kCols, LANES = S::kLanes, GROUPS = S::kGroups;
+    constexpr int PER = TOGETHER ? 1 : GROUPS;          // rows of a wavefront
+    constexpr int SHARE = kWave / PER;                  // lanes that share a row
+    constexpr int STEP = TOGETHER ? GROUPS * kWaves : 1;
     __shared__ f4 sums[kWaves - 1][LANES];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const unsigned unit = together ? blockIdx.x : blockIdx.x * kWaves + wave;
-    const unsigned row = unit / (D / COLS), col = unit % (D / COLS) * COLS + lane % LANES * 4;
-    const int t = (int)(row / p.heads), head = (int)(row % p.heads);
-    if (t >= p.batch.tokens) return;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, group = lane / LANES;
+    const unsigned by_token = (p.heads + PER - 1) / PER * (D / COLS);
+    const unsigned unit = TOGETHER ? blockIdx.x : blockIdx.x * kWaves + wave;
+    const unsigned t0 = unit / by_token, rest = unit % by_token;
+    if (t0 >= (unsigned)p.batch.tokens) return;
+    const int t = __builtin_amdgcn_readfirstlane((int)t0);
+    const int heads0 = (int)(rest / (D / COLS)) * PER + (TOGETHER ? 0 : group);
+    const int head = min(heads0, p.heads - 1), col = (int)(rest % (D / COLS)) * COLS + lane % LANES * 4;
     const int b = token_sequence(p.batch, t);
     if (b >= p.batch.batch) return;
     const Sequence s = sequence(p.batch, b);
@@ -117,46 +138,47 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(AttendParams p, int pr
     const int n = s.seen(t, p.causal);
     if (p.slot == 0 && (p.splits == 1 || n <= p.chunk)) return;  // stored already
     const int own = min((n + p.chunk - 1) / p.chunk, p.splits);
-    const int parts = prefix_parts + own;
-    const size_t at = (size_t)row * p.slots;
+    const int parts = prefix_parts + own, me = lane % SHARE;
+    const size_t at = ((size_t)t * p.heads + head) * p.slots;
     float top = -INFINITY;
-    for (int i = lane; i < parts; i += kWave) top = fmaxf(top, p.ml[at + i].x);
-    top = wave_max(top);
+    for (int i = me; i < parts; i += SHARE) top = fmaxf(top, p.ml[at + i].x);
+#pragma unroll
+    for (int o = 1; o < SHARE; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
     const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
     f4 x = {0, 0, 0, 0};
-    const int first = lane / LANES + (together ? wave * GROUPS : 0);
-    const int step = GROUPS * (together ? kWaves : 1);
-    for (int from = 0; from < parts; from += kWave) {
+    const int first = TOGETHER ? group + wave * GROUPS : 0;
+    for (int from = 0; from < parts; from += SHARE) {
         float weight = 0.0f;
-        if (from + lane < parts) {
-            const float2 ml = p.ml[at + from + lane];
+        if (from + me < parts) {
+            const float2 ml = p.ml[at + from + me];
             weight = fast_exp2(ml.x - ref);
             sum += weight * ml.y;
         }
-        const int count = min(kWave, parts - from);
+        const int count = min(SHARE, parts - from);
 #pragma unroll 4
-        for (int i = first; i - first < count; i += step) {
+        for (int i = first; i - first < count; i += STEP) {
             const int one = min(i, count - 1);
-            const float w = __shfl(weight, one);
+            const float w = __shfl(weight, lane - me + one);
             const f4 part = *(const f4*)(p.po + (at + from + one) * D + col);
             if (i < count) x += w * part;
         }
     }
-    sum = wave_sum(sum);
+#pragma unroll
+    for (int o = 1; o < SHARE; o *= 2) sum += __shfl_xor(sum, o);
     if (s.bad) sum = NAN;
+    if constexpr (TOGETHER) {
 #pragma unroll
-    for (int o = LANES; o < kWave; o *= 2)
+        for (int o = LANES; o < kWave; o *= 2)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], o);
-    if (together) {
+            for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], o);
         if (wave > 0 && lane < LANES) sums[wave - 1][lane] = x;
         __syncthreads();
-        if (wave > 0) return;
+        if (wave > 0 || lane >= LANES) return;
 #pragma unroll
-        for (int w = 0; w + 1 < kWaves; ++w) x += sums[w][lane % LANES];
+        for (int w = 0; w + 1 < kWaves; ++w) x += sums[w][lane];
     }
-    if (lane < LANES) {
+    if (heads0 < p.heads) {
         Piece4<T> y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) y.e[e] = (T)(x[e] / sum);
@@ -172,19 +194,18 @@ struct Range {
 };
 constexpr int kMaxSplits = 256;
 
-// `keys` keys in about `s` ranges, each of `step` keys or more.  `deal`: of a number
-// that lets the streams of kv kv heads deal onto the XCDs (find_item).
-static Range ranges(long long s, int keys, int step, int kv, bool deal) {
-    s = std::min<long long>(s, keys / step);
-    s = std::max<long long>(1, std::min<long long>(s, kMaxSplits));
-    if (deal) {
+// `keys` keys in about `s` ranges, each of whole `step` keys.  deal > 0: of a number
+// that lets the streams of `deal` kv heads deal onto the XCDs (find_item).
+static Range ranges(long long s, int keys, int step, int deal) {
+    s = std::max<long long>(1, std::min<long long>(std::min(s, (long long)kMaxSplits), keys / step));
+    if (deal > 0) {
         int by = kNumXcd;
-        while (by > 1 && (long long)kv * by / 2 % kNumXcd == 0) by /= 2;
+        while (by > 1 && (long long)deal * by / 2 % kNumXcd == 0) by /= 2;
         if (s > by) s -= s % by;
     }
     long long chunk = (keys + s - 1) / s;
     chunk = std::max<long long>(step, (chunk + step - 1) / step * step);
-    if (!deal) s = std::max<long long>(1, (keys + chunk - 1) / chunk);
+    if (deal == 0) s = std::max<long long>(1, (keys + chunk - 1) / chunk);
     return {(int)s, (int)chunk};
 }
 
@@ -206,9 +227,10 @@ struct Plan {
 // of 128, take 214 us in ranges of 1 MiB, 232 in ranges of 2.  Up to 256 KiB stay
 // whole even on an idle device: 784 keys of 64 take 9.7 us whole and 13.4 in seven
 // parts with the merge, 3,000 take 20.8 and 12.6.
-//   Several row tiles: a workgroup a CU; of tile_item four, against unlike lengths
-// (six prompt pieces of 106 .. 700 tokens, kv heads of 64: 83 us with two, 75 with
-// four and ten; a prompt of 4,096, heads of 128: 153 with two and four, 196 with ten).
+//   Several row tiles: a workgroup a CU; of tile_item as many as the device holds at
+// once.  (12 heads on 4 kv heads of 128: six pieces of 400 tokens over 4,000 keys take
+// 101, 87, 105 and 97 us in 1, 2, 3 and 4 ranges, 2 being what it holds; 32 on 8: one
+// of 500 over 6,000 keys 142, 87, 80, 72, 86 in 1 .. 5, 4 being it.)
 //   The prefix: a workgroup a CU (32 tokens over 16,384 keys, 8 kv heads of 128: 37
 // us, 46 with two, 50 with three: more parts to merge).
 template <typename T, int D>
@@ -235,20 +257,25 @@ static Plan plan(const Attention& a) {
                        : (int)std::min<long long>(rows / height + a.batch.batch,
                                                   (most + height - 1) / height * a.batch.batch);
     const long long items = std::max<long long>(1, (long long)p.tiles * kv);
-    long long s = (tile && p.many && !p.single ? 4 : 1) * cu / items;
+    long long s = (tile && p.many && !p.single ? F::kResident : 1) * cu / items;
     if (p.single) {
         const long long by_size = a.max_kv * row / ((D > 256 ? 3LL : 1LL) << 20);
         s = std::max(s, std::min(by_size, 16 * cu / items));
         if (a.max_kv * row <= 256 << 10) s = 1;
     }
-    p.own = ranges(s, a.max_kv, tile && p.many ? 2 * F::kManyKeys : F::kFewKeys, kv, !p.single);
+    const auto divide = [&](long long s, int keys, bool many, bool deal) {
+        // where tile_item works, its matrix instructions bound it, not what L2 misses
+        return tile && many ? ranges(s, keys, 2 * F::kManyKeys, 0)
+                            : ranges(s, keys, F::kFewKeys, deal ? kv : 0);
+    };
+    p.own = divide(s, a.max_kv, p.many, !p.single);
     p.prefix_many = F::kMany && enough && rows >= F::kFrom;
     const int prefix_height = p.prefix_many ? F::kHeight : kRows;
     p.prefix_tiles = (int)((rows + prefix_height - 1) / prefix_height);
     p.prefix = Range{0, 1};
     if (a.prefix_len > 0)
-        p.prefix = ranges(cu / std::max<long long>(1, (long long)p.prefix_tiles * kv),
-                          a.prefix_len, tile && p.prefix_many ? 2 * F::kManyKeys : F::kFewKeys, kv, true);
+        p.prefix = divide(cu / std::max<long long>(1, (long long)p.prefix_tiles * kv),
+                          a.prefix_len, p.prefix_many, true);
     return p;
 }
 
@@ -297,9 +324,11 @@ static void go(const Attention& a, const Plan& plan, void* scratch, hipStream_t 
     p.splits = plan.prefix.splits;
     p.chunk = plan.prefix.chunk;
     p.slot = 0;
-    const long long units = (long long)own.batch.tokens * own.heads * (D > 256 ? D / 256 : 1);
-    const bool together = units < 8 * device_cu_count();
-    const unsigned merge = (unsigned)(together ? units : (units + kWaves - 1) / kWaves);
+    typedef MergeShape<D> M;
+    const int tokens = own.batch.tokens;
+    const bool together = (long long)tokens * own.heads * (D / M::kCols) < 8 * device_cu_count();
+    const long long units = M::units(tokens, own.heads, together);
+    const long long merge = together ? units : (units + kWaves - 1) / kWaves;
     if (!grid_fits("cache attention", blocks(p) + blocks(own)) ||
         !grid_fits("cache attention", merge))
         return;
@@ -320,8 +349,11 @@ static void go(const Attention& a, const Plan& plan, void* scratch, hipStream_t 
         if constexpr (F::kMany)
             cache_attend_kernel<T, D, true><<<(unsigned)blocks(own), 256, 0, stream>>>(own);
     }
-    if (own.po)
-        cache_merge_kernel<T, D><<<merge, 256, 0, stream>>>(own, own.slot, together);
+    if (!own.po) return;
+    if (together)
+        cache_merge_kernel<T, D, true><<<(unsigned)merge, 256, 0, stream>>>(own, own.slot);
+    else
+        cache_merge_kernel<T, D, false><<<(unsigned)merge, 256, 0, stream>>>(own, own.slot);
 }
 
 // f(T{}, dim as a constant) for the call's type and dim.

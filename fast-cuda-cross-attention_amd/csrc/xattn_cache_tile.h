@@ -13,7 +13,7 @@
 // type.
 //
 // Bound by the matrix pipe: a causal prompt of 4,096 tokens, 32 heads on 8 kv heads
-// of 128, takes 151 us, 911 TFLOP/s of what the mask leaves (of 1,167 in a large
+// of 128, takes 147 us, 935 TFLOP/s of what the mask leaves (of 1,167 in a large
 // matrix product); heads of 256 run at about 290, with a half of the rows to an
 // operand and one wavefront's registers full.
 #pragma once

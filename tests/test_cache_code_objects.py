@@ -18,7 +18,7 @@ def test_every_form_is_there_once(device_asm):
     names = [n for n in _bodies(device_asm) if "5cache" in n]
     assert sum("cache_attend_kernel" in n for n in names) == ATTEND
     assert sum("cache_prefix_kernel" in n for n in names) == PREFIX
-    assert sum("cache_merge_kernel" in n for n in names) == 12
+    assert sum("cache_merge_kernel" in n for n in names) == 12 * 2
     assert sum("rope_kernel" in n for n in names) == 3 * 2 * 2
     assert sum("cache_append_kernel" in n for n in names) == 3 * 2 * 2
 
