@@ -5,17 +5,18 @@
 // Each of the four wavefronts holds RB blocks of sixteen rows; all share tiles of K
 // and V in LDS, so an operand read from LDS feeds RB matrix instructions.  There are
 // two of each tile: DMA fills one pair, piece by piece between the matrix
-// instructions, while the other is worked on; one barrier a tile.  Two
-// workgroups share a CU, so that one's softmax goes beside the other's products, whose
-// wavefronts go first (s_setprio).  Weights are taken relative to a maximum that is
-// renewed only when a score exceeds it by kLag (in exponents of 2), so that the
-// output is rarely rescaled; they stay below 2^kLag, far from the range of either
-// type.
+// instructions, while the other is worked on; one barrier a tile.  Two workgroups
+// share a CU (three at 64), and the wavefronts at their scores go before those at
+// their softmax (s_setprio: 151 us in the case below, 163 without, 158 for the product
+// with V as well).  Weights are taken relative to a maximum that is renewed only when a
+// score exceeds it by kLag (in exponents of 2), so that the output is rarely rescaled;
+// they stay below 2^kLag, far from the range of either type.
 //
-// Bound by the matrix pipe: a causal prompt of 4,096 tokens, 32 heads on 8 kv heads
-// of 128, takes 147 us, 935 TFLOP/s of what the mask leaves (of 1,167 in a large
-// matrix product); heads of 256 run at about 290, with a half of the rows to an
-// operand and one wavefront's registers full.
+// Bound by the issue of matrix and vector instructions, which fill 45 % and 54 % of a
+// SIMD's cycles in a causal prompt of 4,096 tokens, 32 heads on 8 kv heads of 128:
+// 147 us, 935 TFLOP/s of what the mask leaves (a large matrix product: 1,167).  At 64
+// half the matrix instructions meet the same number of weights: eight sequences of
+// 2,048 tokens over 4,096 keys run at 695, at 128 at 872.
 #pragma once
 
 #include "xattn_cache_item.h"

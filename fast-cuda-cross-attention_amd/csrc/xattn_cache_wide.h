@@ -25,6 +25,12 @@
 //
 // The waits count the DMA by themselves, so no other load may stand between: the
 // pages of 64 tiles are looked up at a time.
+//
+// Few rows are bound by memory (32 sequences of 4,000 keys, one token each: 5.2 to 5.6
+// TB/s at all dims), many by the matrix instructions and what the wavefront does
+// between them: 64 rows over 50,176 keys of 768 take 122 us with the matrix pipe busy
+// for 57 % of them, 1,024 tokens over 1,500 keys run at 67 TFLOP/s at 64, 82 at 128, 68
+// at 256 (a large matrix product: 153).
 #pragma once
 
 #include "xattn_cache_item.h"

@@ -899,6 +899,15 @@ def _decode(x, precision):
     return x.astype(np.float32)
 
 
+def _int32(x, what):
+    """x as a contiguous int32 array; ValueError if that would change a value."""
+    host = np.asarray(x)
+    if host.size and (host.dtype.kind not in "iu" or host.min() < -2 ** 31
+                      or host.max() >= 2 ** 31):
+        raise ValueError(f"{what} are not 32-bit integers")
+    return np.ascontiguousarray(host, np.int32)
+
+
 def _bits_type(precision):
     return {"fp32": np.float32, "fp16": np.float16, "bf16": np.uint16}[precision]
 
@@ -952,8 +961,10 @@ def run_rope(x, positions, rope, inverse=False, precision="fp32"):
     _require_cache()
     code = _precision(precision)
     host = _encode(np.asarray(x, np.float32), precision)
+    if host.ndim != 3:
+        raise ValueError(f"x of shape {host.shape} is not [tokens, heads, dim]")
     tokens, heads, dim = host.shape
-    positions = np.ascontiguousarray(positions, np.int32)
+    positions = _int32(positions, "positions")
     if positions.shape != (tokens,):
         raise ValueError(f"positions of shape {positions.shape} for {tokens} tokens")
     with DeviceBuffer.holding(host) as dx, DeviceBuffer(host.nbytes) as dy, \
@@ -1008,8 +1019,8 @@ class PagedCache:
                      for b in (self._k, self._v))
 
     def _batch(self, owned, tokens, q_starts, kv_lens, page_table):
-        q_starts, kv_lens = (np.ascontiguousarray(a, np.int32) for a in (q_starts, kv_lens))
-        page_table = np.ascontiguousarray(page_table, np.int32)
+        q_starts, kv_lens = _int32(q_starts, "q_starts"), _int32(kv_lens, "kv_lens")
+        page_table = _int32(page_table, "page_table's entries")
         batch = kv_lens.size
         if q_starts.shape != (batch + 1,) or page_table.ndim != 2 or len(page_table) != batch:
             raise ValueError(f"q_starts {q_starts.shape}, kv_lens {kv_lens.shape} and page_table "
@@ -1034,7 +1045,7 @@ class PagedCache:
         if len(v) != len(k) or (q is not None and len(q) != len(k)):
             raise ValueError("k, v and q have to hold the same tokens")
         if positions is not None:
-            positions = np.ascontiguousarray(positions, np.int32)
+            positions = _int32(positions, "positions")
             if positions.shape != (len(k),):
                 raise ValueError(f"positions of shape {positions.shape} for {len(k)} tokens")
         row = self.shape[1] * self.shape[3]
@@ -1069,7 +1080,7 @@ class PagedCache:
             batch = self._batch(owned, tokens, q_starts, kv_lens, page_table)
             launch, before, prefix = lib.launch_cache_attention_kernel, (), None
             if prefix_pages is not None:
-                prefix_pages = np.ascontiguousarray(prefix_pages, np.int32)
+                prefix_pages = _int32(prefix_pages, "prefix_pages")
                 on = owned.enter_context(DeviceBuffer.holding(prefix_pages))
                 prefix = ctypes.byref(PrefixArgs(on.ptr.value, prefix_pages.size, prefix_len))
                 launch, before = lib.launch_prefix_attention_kernel, (prefix,)

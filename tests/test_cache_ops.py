@@ -276,3 +276,21 @@ def test_work_is_not_divided_without_need(cw):
     assert need(tokens=1, batch=1, max_q_len=1, max_kv_len=60000, table_width=10000) > 0
     assert need(tokens=4096, batch=4096, max_q_len=1, max_kv_len=60000, table_width=10000) == 0
     assert cw.HAS_CACHE
+
+
+@pytest.mark.parametrize("q_starts, kv_lens, table", [
+    ([0, 1], [2 ** 32 + 1], [[0]]), ([0, 1], [1], [[2 ** 31]]), ([0, 1], [1.5], [[0]]),
+    ([0, -2 ** 31 - 1], [1], [[0]])])
+def test_host_api_takes_no_other_integers(cw, q_starts, kv_lens, table):
+    """Numbers that 32 bits would change are refused, not wrapped."""
+    cache = object.__new__(cw.PagedCache)  # no device memory behind it
+    cache.shape, cache.precision, cache.code = (4, 2, 16, 64), "fp32", 0
+    x = np.zeros((1, 2, 64), np.float32)
+    with pytest.raises(ValueError, match="32-bit"):
+        cache.append(x, x, q_starts, kv_lens, table)
+    with pytest.raises(ValueError, match="32-bit"):
+        cache.append(x, x, [0, 1], [1], [[0]], positions=[2 ** 31])
+    with pytest.raises(ValueError, match="32-bit"):
+        cw.run_rope(x, [2 ** 31], object.__new__(cw.Rope))
+    with pytest.raises(ValueError, match="tokens, heads, dim"):
+        cw.run_rope(x[0], [0], object.__new__(cw.Rope))
