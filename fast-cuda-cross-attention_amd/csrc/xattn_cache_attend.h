@@ -101,7 +101,7 @@ cache_prefix_kernel(AttendParams prefix, AttendParams own, unsigned prefix_block
 // rows of many parts (TOGETHER): a workgroup a row, its groups of LANES lanes taking
 // every so many-th part.  Otherwise a group a row, those of a wavefront heads of
 // one token: what a row waits for are four reads one after another (its sequence,
-// length, maxima, parts), so many rows have to wait at once (20,860 rows of up to
+// length, maxima, parts), so many rows have to wait at once (26,076 rows of up to
 // four parts of 64: 13.0 us with a wavefront a row, 7.4 with a group).
 // --------------------------------------------------------------------------
 template <int D>
@@ -284,8 +284,22 @@ static size_t parts(const Attention& a, const Plan& p) {
     return (size_t)a.batch.tokens * a.heads * p.slots();
 }
 
-static long long blocks(const AttendParams& p) {
-    return (long long)p.pages.kv_heads * p.tiles * p.splits;
+// Workgroups of the launches: the prefix's, those and the sequences' own, the merge's.
+struct Grid {
+    long long first, all, merge;
+    bool together;
+};
+
+template <int D>
+static Grid grid(const Attention& a, const Plan& plan) {
+    const long long kv = a.pages.kv_heads;
+    Grid g;
+    g.first = kv * plan.prefix_tiles * plan.prefix.splits;
+    g.all = g.first + kv * plan.tiles * plan.own.splits;
+    g.together = MergeShape<D>::units(a.batch.tokens, a.heads, true) < 8 * device_cu_count();
+    const long long units = MergeShape<D>::units(a.batch.tokens, a.heads, g.together);
+    g.merge = parts(a, plan) == 0 ? 0 : g.together ? units : (units + kWaves - 1) / kWaves;
+    return g;
 }
 
 template <typename T, int D>
@@ -318,22 +332,16 @@ static void go(const Attention& a, const Plan& plan, void* scratch, hipStream_t 
         own.po = (float*)scratch;
         own.ml = (float2*)(own.po + n * D);
     }
-    AttendParams p = own;
-    p.single = 0;
-    p.tiles = plan.prefix_tiles;
-    p.splits = plan.prefix.splits;
-    p.chunk = plan.prefix.chunk;
-    p.slot = 0;
-    typedef MergeShape<D> M;
-    const int tokens = own.batch.tokens;
-    const bool together = (long long)tokens * own.heads * (D / M::kCols) < 8 * device_cu_count();
-    const long long units = M::units(tokens, own.heads, together);
-    const long long merge = together ? units : (units + kWaves - 1) / kWaves;
-    if (!grid_fits("cache attention", blocks(p) + blocks(own)) ||
-        !grid_fits("cache attention", merge))
-        return;
-    if (plan.prefix.splits > 0) {
-        const unsigned first = (unsigned)blocks(p), all = first + (unsigned)blocks(own);
+    const Grid g = grid<D>(a, plan);
+    if (!grid_fits("cache attention", std::max(g.all, g.merge))) return;
+    const unsigned first = (unsigned)g.first, all = (unsigned)g.all;
+    if (first > 0) {
+        AttendParams p = own;
+        p.single = 0;
+        p.tiles = plan.prefix_tiles;
+        p.splits = plan.prefix.splits;
+        p.chunk = plan.prefix.chunk;
+        p.slot = 0;
         // a sequence has no more rows than the batch
         if constexpr (F::kMany) {
             if (plan.many)
@@ -344,16 +352,15 @@ static void go(const Attention& a, const Plan& plan, void* scratch, hipStream_t 
         if (!plan.prefix_many)
             cache_prefix_kernel<T, D, false, false><<<all, 256, 0, stream>>>(p, own, first);
     } else if (!plan.many) {
-        cache_attend_kernel<T, D, false><<<(unsigned)blocks(own), 256, 0, stream>>>(own);
+        cache_attend_kernel<T, D, false><<<all, 256, 0, stream>>>(own);
     } else {
-        if constexpr (F::kMany)
-            cache_attend_kernel<T, D, true><<<(unsigned)blocks(own), 256, 0, stream>>>(own);
+        if constexpr (F::kMany) cache_attend_kernel<T, D, true><<<all, 256, 0, stream>>>(own);
     }
-    if (!own.po) return;
-    if (together)
-        cache_merge_kernel<T, D, true><<<(unsigned)merge, 256, 0, stream>>>(own, own.slot);
-    else
-        cache_merge_kernel<T, D, false><<<(unsigned)merge, 256, 0, stream>>>(own, own.slot);
+    const unsigned merge = (unsigned)g.merge;
+    if (merge > 0 && g.together)
+        cache_merge_kernel<T, D, true><<<merge, 256, 0, stream>>>(own, own.slot);
+    else if (merge > 0)
+        cache_merge_kernel<T, D, false><<<merge, 256, 0, stream>>>(own, own.slot);
 }
 
 // f(T{}, dim as a constant) for the call's type and dim.
@@ -373,7 +380,11 @@ static void dispatch(const Attention& a, F f) {
 size_t attention_scratch(const Attention& a) {
     size_t n = 0;
     dispatch(a, [&](auto type, auto dim) {
-        n = parts(a, plan<decltype(type), dim()>(a)) * (dim() * sizeof(float) + sizeof(float2));
+        constexpr int D = dim();
+        const Plan p = plan<decltype(type), D>(a);
+        const Grid g = grid<D>(a, p);
+        if (std::max(g.all, g.merge) <= kMaxBlocks)  // else the launch refuses
+            n = parts(a, p) * (D * sizeof(float) + sizeof(float2));
     });
     return n;
 }

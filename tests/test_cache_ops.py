@@ -275,6 +275,7 @@ def test_work_is_not_divided_without_need(cw):
     assert need(tokens=1, batch=1, max_q_len=1, max_kv_len=60) == 0
     assert need(tokens=1, batch=1, max_q_len=1, max_kv_len=60000, table_width=10000) > 0
     assert need(tokens=4096, batch=4096, max_q_len=1, max_kv_len=60000, table_width=10000) == 0
+    assert need(tokens=1 << 27, batch=1 << 27, max_q_len=1, max_kv_len=60000) == 0  # refused
     assert cw.HAS_CACHE
 
 
